@@ -256,8 +256,8 @@ def _own_logprobs(state: dict):
     if case["top_k"]:
         outputs += [r.top_ids, r.top_logprobs]
     if case["grad"]:
-        outputs.append(ops.token_logprobs_backward(state["logits"], state["targets"], r.lse, r.entropy,
-                                                   state["d_logprobs"], state["d_entropy"], ignore_index=_IGNORED))
+        outputs.append(ops.token_logprobs_backward(state["logits"], state["targets"], r, state["d_logprobs"],
+                                                   state["d_entropy"], ignore_index=_IGNORED))
     return outputs
 
 
