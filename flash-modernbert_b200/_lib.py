@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 from .errors import PackedEncodersError
@@ -110,6 +110,20 @@ PROTOTYPES = {
                                c_void_p, c_size_t, c_void_p, c_void_p]),
     "pe_attn_varlen_static": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p,
                                       c_void_p, c_void_p]),
+    "pe_attn_varlen_lse": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p,
+                                   c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "pe_attn_backward_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "pe_attn_varlen_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
+                                        c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                        c_size_t, c_void_p, c_void_p]),
+    "pe_dropout": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_double, c_void_p, c_void_p, c_void_p,
+                           c_void_p]),
+    "pe_token_logprobs": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                  c_void_p]),
+    "pe_token_logprobs_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                           c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                           c_void_p, c_int64, c_void_p]),
     "pe_forward_workspace_bytes": (c_size_t, [POINTER(PeModel), c_int64, c_int]),
     "pe_forward_packed": (c_int, [POINTER(PeModel), c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                   c_int, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),

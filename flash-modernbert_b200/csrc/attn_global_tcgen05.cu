@@ -185,10 +185,14 @@ __device__ __noinline__ GByHand g_tile_by_hand(const __nv_bfloat16* qrow, const 
   return GByHand{m_ref, l_run, sum};
 }
 
+// LSE: the natural logarithm of each row's sum of exponentials is stored too (lse [nh, T]), for a
+// backward pass; the inference form carries no code for it.
+template <bool LSE>
 __global__ void __launch_bounds__(G_THREADS, 2)
 attn_global_tc_kernel(const __grid_constant__ CUtensorMap tm_qkv, const int4* __restrict__ tile_info,
                       const int32_t* __restrict__ total_tiles_ptr, int nh, int half_window,
-                      const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ out, int* status) {
+                      const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ out,
+                      float* __restrict__ lse, int64_t T, int* status) {
   const int total_items = *total_tiles_ptr * nh;
   if (int(blockIdx.x) >= total_items) return;  // whole CTA leaves before any barrier or allocation
 
@@ -495,6 +499,8 @@ attn_global_tc_kernel(const __grid_constant__ CUtensorMap tm_qkv, const int4* __
         wait(bar(GB_O_FULL), (g - 1) & 1);
         tc_fence_after();
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        if (LSE && ok && qi < it.len)  // l_run is in units of 2^m_ref
+          lse[it.head * T + it.seq_begin + qi] = (m_ref + log2f(l_run)) * 0.69314718055994530942f;
         __nv_bfloat16* orow = out + (int64_t(it.seq_begin) + qi) * H + it.head * 64;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -529,9 +535,10 @@ attn_global_tc_kernel(const __grid_constant__ CUtensorMap tm_qkv, const int4* __
 }
 
 int attn_run_global_tc(const void* qkv, const int4* tile_info, const int32_t* total_tiles,
-                       int64_t max_tiles, int64_t T, int nh, int half_window, void* out,
+                       int64_t max_tiles, int64_t T, int nh, int half_window, void* out, float* lse,
                        int32_t* status, cudaStream_t st) {
-  int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(attn_global_tc_kernel), G_SMEM, true);
+  auto kern = lse != nullptr ? attn_global_tc_kernel<true> : attn_global_tc_kernel<false>;
+  int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), G_SMEM, true);
   if (rc != PE_OK) return rc;
   CUtensorMap tm;
   rc = make_tmap_bf16_2d(&tm, qkv, (uint64_t)T, (uint64_t)(3 * nh * 64), (uint64_t)(3 * nh * 64),
@@ -540,9 +547,9 @@ int attn_run_global_tc(const void* qkv, const int4* tile_info, const int32_t* to
   const int64_t max_items = max_tiles * nh;
   const int64_t slots = 2 * (int64_t)sm_count();  // two resident CTAs per SM
   const int grid = (int)(max_items < slots ? max_items : slots);
-  attn_global_tc_kernel<<<grid, G_THREADS, G_SMEM, st>>>(tm, tile_info, total_tiles, nh, half_window,
-                                                        static_cast<const __nv_bfloat16*>(qkv),
-                                                        static_cast<__nv_bfloat16*>(out), status);
+  kern<<<grid, G_THREADS, G_SMEM, st>>>(tm, tile_info, total_tiles, nh, half_window,
+                                        static_cast<const __nv_bfloat16*>(qkv),
+                                        static_cast<__nv_bfloat16*>(out), lse, T, status);
   PE_LAUNCH_CHECK("attn_global_tc_kernel");
   return PE_OK;
 }

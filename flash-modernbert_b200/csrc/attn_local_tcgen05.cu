@@ -71,10 +71,13 @@ __device__ __forceinline__ LwItem lw_item(const int4* __restrict__ tile_info, in
   return it;
 }
 
+// LSE: the natural logarithm of each row's sum of exponentials is stored too (lse [nh, T]), for a
+// backward pass; the inference form carries no code for it.
+template <bool LSE>
 __global__ void __launch_bounds__(LW_THREADS, 2)
 attn_local_tc2_kernel(const __grid_constant__ CUtensorMap tm_qkv, const int4* __restrict__ tile_info,
                       const int32_t* __restrict__ total_tiles_ptr, int nh,
-                      __nv_bfloat16* __restrict__ out, int* status) {
+                      __nv_bfloat16* __restrict__ out, float* __restrict__ lse, int64_t T, int* status) {
   const int total_items = *total_tiles_ptr * nh;
   if (int(blockIdx.x) >= total_items) return;  // whole CTA leaves before any barrier or allocation
 
@@ -376,6 +379,8 @@ attn_local_tc2_kernel(const __grid_constant__ CUtensorMap tm_qkv, const int4* __
       wait(bar(LB_O_FULL), n & 1);
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (LSE && ok && qi < len)  // l is in units of 2^m_safe
+        lse[this_head * T + seq_begin + qi] = (m_safe + log2f(l)) * 0.69314718055994530942f;
       uint32_t o0[32], o1[32];
       g_tmem_ld32(lane_addr + LW_O_COL, o0);
       g_tmem_ld32(lane_addr + LW_O_COL + 32, o1);
@@ -423,9 +428,10 @@ attn_local_tc2_kernel(const __grid_constant__ CUtensorMap tm_qkv, const int4* __
 }
 
 int attn_run_local_tc2(const void* qkv, const int4* tile_info, const int32_t* total_tiles,
-                       int64_t max_tiles, int64_t T, int nh, void* out, int32_t* status,
+                       int64_t max_tiles, int64_t T, int nh, void* out, float* lse, int32_t* status,
                        cudaStream_t st) {
-  int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(attn_local_tc2_kernel), LW_SMEM, true);
+  auto kern = lse != nullptr ? attn_local_tc2_kernel<true> : attn_local_tc2_kernel<false>;
+  int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), LW_SMEM, true);
   if (rc != PE_OK) return rc;
   CUtensorMap tm;
   rc = make_tmap_bf16_2d(&tm, qkv, (uint64_t)T, (uint64_t)(3 * nh * 64), (uint64_t)(3 * nh * 64),
@@ -434,8 +440,8 @@ int attn_run_local_tc2(const void* qkv, const int4* tile_info, const int32_t* to
   const int64_t max_items = max_tiles * nh;
   const int64_t slots = 2 * (int64_t)sm_count();  // two resident CTAs per SM
   const int grid = (int)(max_items < slots ? max_items : slots);
-  attn_local_tc2_kernel<<<grid, LW_THREADS, LW_SMEM, st>>>(tm, tile_info, total_tiles, nh,
-                                                          static_cast<__nv_bfloat16*>(out), status);
+  kern<<<grid, LW_THREADS, LW_SMEM, st>>>(tm, tile_info, total_tiles, nh,
+                                          static_cast<__nv_bfloat16*>(out), lse, T, status);
   PE_LAUNCH_CHECK("attn_local_tc2_kernel");
   return PE_OK;
 }

@@ -37,10 +37,27 @@ constexpr int ATT_D = 64;
 // clamped into range and reported as ST_BAD_CU_SEQLENS, and no more than `cap_long` main tiles are
 // written, so that neither this kernel nor the ones that follow the descriptors can leave the
 // caller's buffers.
+// Blocks past the first (launched only with `tail_out`, for a forward whose gradient is taken) write
+// the rows that no sequence holds, which the attention kernels leave alone: zeros in tail_out
+// [T, nh * 64] and -inf, the logarithm of an empty sum, in tail_lse [nh, T].
 __global__ void attn_schedule_kernel(const int32_t* __restrict__ cu_seqlens, int n_seqs, int T, int bm,
                                      int short_max, int cap_long, int32_t* __restrict__ tile_start,
                                      int32_t* __restrict__ short_start, int4* __restrict__ tile_info,
-                                     int4* __restrict__ short_info, int* status) {
+                                     int4* __restrict__ short_info, uint4* __restrict__ tail_out,
+                                     float* __restrict__ tail_lse, int nh, int* status) {
+  if (blockIdx.x > 0) {
+    const int head_end = min(max(cu_seqlens[0], 0), T), tail_begin = min(max(cu_seqlens[n_seqs], 0), T);
+    const int64_t first = int64_t(blockIdx.x - 1) * blockDim.x + threadIdx.x;
+    const int64_t step = int64_t(gridDim.x - 1) * blockDim.x;
+    for (int part = 0; part < 2; ++part) {
+      const int row0 = part == 0 ? 0 : tail_begin, rows = part == 0 ? head_end : T - tail_begin;
+      for (int64_t i = first; i < int64_t(rows) * nh * 8; i += step)
+        tail_out[int64_t(row0) * nh * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int64_t i = first; i < int64_t(rows) * nh; i += step)
+        tail_lse[(i / rows) * T + row0 + i % rows] = -INFINITY;
+    }
+    return;
+  }
   __shared__ unsigned long long warp_sums[32];
   __shared__ unsigned long long carry_s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -164,11 +181,12 @@ __device__ __forceinline__ void load_tile_async(uint32_t smem_tile, const __nv_b
   }
 }
 
-template <int NWARPS>
+// LSE: the natural logarithm of each row's sum of exponentials is stored too (lse [nh, T]).
+template <int NWARPS, bool LSE>
 __global__ void __launch_bounds__(NWARPS * 32, 16 / NWARPS)  // 16 warps per SM: 128 registers
 attn_varlen_mma_kernel(const __nv_bfloat16* __restrict__ qkv, const int4* __restrict__ tile_info,
                        const int32_t* __restrict__ total_tiles_ptr, int nh, int half_window,
-                       __nv_bfloat16* __restrict__ out) {
+                       __nv_bfloat16* __restrict__ out, float* __restrict__ lse, int64_t T) {
   constexpr int BM = NWARPS * 16;
   constexpr int THREADS = NWARPS * 32;
   // One CTA serves a query tile for several heads (blockIdx.y, blockIdx.y + gridDim.y, ...), with
@@ -399,6 +417,12 @@ attn_varlen_mma_kernel(const __nv_bfloat16* __restrict__ qkv, const int4* __rest
   // normalise, stage this warp's 16 x 64 outputs in its own rows of the Q tile, store 16 B wide
   const float inv0 = l_run[0] > 0.f ? 1.f / l_run[0] : 0.f;
   const float inv1 = l_run[1] > 0.f ? 1.f / l_run[1] : 0.f;
+  if (LSE && active && (lane & 3) == 0) {  // l_run is in units of 2^m_run
+#pragma unroll
+    for (int h2 = 0; h2 < 2; ++h2)
+      if (qrow0 + h2 * 8 < len)
+        lse[head * T + seq_begin + qrow0 + h2 * 8] = (m_run[h2] + log2f(l_run[h2])) * 0.69314718055994530942f;
+  }
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -466,30 +490,35 @@ static TileTables tile_tables(void* scratch, int n_seqs, int64_t T, int bm) {
 }
 
 int attn_schedule(const int32_t* cu_seqlens, int n_seqs, int64_t T, int bm, bool split_short,
-                  void* scratch, int32_t* status, cudaStream_t st) {
+                  void* scratch, int32_t* status, cudaStream_t st, void* tail_out, float* tail_lse, int nh) {
   PE_REQUIRE(T >= 0 && T < (1ll << 31) - 256 && n_seqs > 0 && T / bm + n_seqs < (1ll << 31),
              "attention schedule: %lld tokens / %d sequences out of range", (long long)T, n_seqs);
   const TileTables t = tile_tables(scratch, n_seqs, T, bm);
-  attn_schedule_kernel<<<1, 1024, 0, st>>>(cu_seqlens, n_seqs, (int)T, bm,
+  attn_schedule_kernel<<<tail_out != nullptr ? 65 : 1, 1024, 0, st>>>(cu_seqlens, n_seqs, (int)T, bm,
                                            split_short ? ATT_SHORT_MAX : 0, t.cap_long, t.tile_start,
-                                           t.short_start, t.tile_info, t.short_info, status);
+                                           t.short_start, t.tile_info, t.short_info,
+                                           static_cast<uint4*>(tail_out), tail_lse, nh, status);
   PE_LAUNCH_CHECK("attn_schedule_kernel");
   return PE_OK;
 }
 
 static int launch_short(const __nv_bfloat16* q, const int4* info, const int32_t* total, int64_t max_tiles,
                         int bm, int nh, int half_window, int heads_per_cta, __nv_bfloat16* o,
-                        cudaStream_t st) {
+                        float* lse, int64_t T, cudaStream_t st) {
   dim3 grid((unsigned)max_tiles, (unsigned)((nh + heads_per_cta - 1) / heads_per_cta));
+  const bool with = lse != nullptr;
   switch (bm) {
     case 16:
-      attn_varlen_mma_kernel<1><<<grid, 32, 0, st>>>(q, info, total, nh, half_window, o);
+      (with ? attn_varlen_mma_kernel<1, true> : attn_varlen_mma_kernel<1, false>)<<<grid, 32, 0, st>>>(
+          q, info, total, nh, half_window, o, lse, T);
       break;
     case 32:
-      attn_varlen_mma_kernel<2><<<grid, 64, 0, st>>>(q, info, total, nh, half_window, o);
+      (with ? attn_varlen_mma_kernel<2, true> : attn_varlen_mma_kernel<2, false>)<<<grid, 64, 0, st>>>(
+          q, info, total, nh, half_window, o, lse, T);
       break;
     case 64:
-      attn_varlen_mma_kernel<4><<<grid, 128, 0, st>>>(q, info, total, nh, half_window, o);
+      (with ? attn_varlen_mma_kernel<4, true> : attn_varlen_mma_kernel<4, false>)<<<grid, 128, 0, st>>>(
+          q, info, total, nh, half_window, o, lse, T);
       break;
     default:
       set_last_error("attention: unsupported query tile %d", bm);
@@ -500,25 +529,26 @@ static int launch_short(const __nv_bfloat16* q, const int4* info, const int32_t*
 }
 
 int attn_run(const void* qkv, const void* scratch, int n_seqs, int64_t T, int nh, int half_window,
-             int bm, void* out, int32_t* status, cudaStream_t st) {
+             int bm, void* out, int32_t* status, cudaStream_t st, float* lse) {
   const TileTables t = tile_tables(const_cast<void*>(scratch), n_seqs, T, bm);
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(qkv);
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
   // A batch of short sequences only: four heads per CTA (see the kernel) - enough CTAs to fill the
   // GPU, few enough that each hides its own load latency.
-  if (bm != 128) return launch_short(q, t.tile_info, t.tile_start + n_seqs, t.cap_long, bm, nh, half_window, 4, o, st);
+  if (bm != 128)
+    return launch_short(q, t.tile_info, t.tile_start + n_seqs, t.cap_long, bm, nh, half_window, 4, o, lse, T, st);
   // Long batch: the tensor-memory kernels take the sequences of more than 64 tokens (at most
   // T / 128 + T / 65 tiles of them exist), the register kernel with 64-row tiles the rest.
   const int64_t max_long = std::min<int64_t>(t.cap_long, T / 128 + T / (ATT_SHORT_MAX + 1) + 1);
   int rc = (half_window == 64)
-               ? attn_run_local_tc2(qkv, t.tile_info, t.tile_start + n_seqs, max_long, T, nh, out, status, st)
+               ? attn_run_local_tc2(qkv, t.tile_info, t.tile_start + n_seqs, max_long, T, nh, out, lse, status, st)
                : attn_run_global_tc(qkv, t.tile_info, t.tile_start + n_seqs, max_long, T, nh, half_window,
-                                    out, status, st);
+                                    out, lse, status, st);
   if (rc != PE_OK) return rc;
   // Usually few sequences are short here, so this launch is a latency chain, not a throughput
   // problem: one head per CTA keeps the chain at a quarter of the four-head form's.
   const int64_t max_short = std::min<int64_t>(n_seqs, T);
-  return launch_short(q, t.short_info, t.short_start + n_seqs, max_short, 64, nh, half_window, 1, o, st);
+  return launch_short(q, t.short_info, t.short_start + n_seqs, max_short, 64, nh, half_window, 1, o, lse, T, st);
 }
 
 // ---- scratch that needs no allocation -------------------------------------------------
@@ -580,24 +610,40 @@ extern "C" size_t pe_attn_workspace_bytes(int64_t T, int n_seqs) {
   return pe::attn_scratch_bytes(T, n_seqs);
 }
 
-extern "C" int pe_attn_varlen(const void* qkv, const int32_t* cu_seqlens, int n_seqs, int64_t T,
-                              int nh, int half_window, int max_seqlen, void* out, void* workspace,
-                              size_t workspace_bytes, int32_t* status, void* stream) {
+// pe_attn_varlen and pe_attn_varlen_lse: `lse` is NULL for the first.
+static int attn_varlen_checked(const void* qkv, const int32_t* cu_seqlens, int n_seqs, int64_t T, int nh,
+                               int half_window, int max_seqlen, void* out, float* lse, void* workspace,
+                               size_t workspace_bytes, int32_t* status, void* stream, const char* who) {
   using namespace pe;
-  PE_REQUIRE(qkv && cu_seqlens && out && workspace, "pe_attn_varlen: null pointer");
-  PE_REQUIRE(n_seqs > 0 && T >= 0 && nh > 0 && nh <= 65535, "pe_attn_varlen: bad sizes");
-  PE_REQUIRE(max_seqlen > 0, "pe_attn_varlen: max_seqlen must be positive");
-  PE_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
-             "pe_attn_varlen: workspace must be 16-byte aligned");
+  PE_REQUIRE(qkv && cu_seqlens && out && workspace, "%s: null pointer", who);
+  PE_REQUIRE(n_seqs > 0 && T >= 0 && nh > 0 && nh <= 65535, "%s: bad sizes", who);
+  PE_REQUIRE(max_seqlen > 0, "%s: max_seqlen must be positive", who);
+  PE_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: workspace must be 16-byte aligned", who);
   if (workspace_bytes < pe_attn_workspace_bytes(T, n_seqs)) {
-    set_last_error("pe_attn_varlen: workspace %zu < %zu bytes", workspace_bytes,
-                   pe_attn_workspace_bytes(T, n_seqs));
+    set_last_error("%s: workspace %zu < %zu bytes", who, workspace_bytes, pe_attn_workspace_bytes(T, n_seqs));
     return PE_ERR_WORKSPACE;
   }
   if (T == 0) return PE_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int bm = attn_pick_bm(max_seqlen);
-  int rc = attn_schedule(cu_seqlens, n_seqs, T, bm, bm == 128, workspace, status, st);
+  int rc = attn_schedule(cu_seqlens, n_seqs, T, bm, bm == 128, workspace, status, st,
+                         lse != nullptr ? out : nullptr, lse, nh);
   if (rc != PE_OK) return rc;
-  return attn_run(qkv, workspace, n_seqs, T, nh, half_window, bm, out, status, st);
+  return attn_run(qkv, workspace, n_seqs, T, nh, half_window, bm, out, status, st, lse);
+}
+
+extern "C" int pe_attn_varlen(const void* qkv, const int32_t* cu_seqlens, int n_seqs, int64_t T,
+                              int nh, int half_window, int max_seqlen, void* out, void* workspace,
+                              size_t workspace_bytes, int32_t* status, void* stream) {
+  return attn_varlen_checked(qkv, cu_seqlens, n_seqs, T, nh, half_window, max_seqlen, out, nullptr, workspace,
+                             workspace_bytes, status, stream, "pe_attn_varlen");
+}
+
+extern "C" int pe_attn_varlen_lse(const void* qkv, const int32_t* cu_seqlens, int n_seqs, int64_t T,
+                                  int nh, int half_window, int max_seqlen, void* out, float* lse,
+                                  void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  PE_REQUIRE(lse != nullptr && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
+             "pe_attn_varlen_lse: lse is NULL or out is not 16-byte aligned");
+  return attn_varlen_checked(qkv, cu_seqlens, n_seqs, T, nh, half_window, max_seqlen, out, lse, workspace,
+                             workspace_bytes, status, stream, "pe_attn_varlen_lse");
 }

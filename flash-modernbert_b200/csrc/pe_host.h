@@ -54,17 +54,20 @@ size_t attn_info_offset(int n_seqs);
 // ST_BAD_CU_SEQLENS in `status` (may be NULL); at most T / bm + n_seqs tiles are written.
 // `split_short` (attention with bm = 128 only) lists sequences of at most 64 tokens in the second
 // table, for the register-tiled kernel; attn_run expects the tables of an attention forward built so.
+// With `tail_out` (and `tail_lse`, `nh`) the rows outside every sequence are set to 0 and -inf.
 int attn_schedule(const int32_t* cu_seqlens, int n_seqs, int64_t T, int bm, bool split_short,
-                  void* scratch, int32_t* status, cudaStream_t st);
+                  void* scratch, int32_t* status, cudaStream_t st, void* tail_out = nullptr,
+                  float* tail_lse = nullptr, int nh = 0);
+// `lse` (may be NULL): float [nh, T], the natural logarithm of every row's sum of exponentials.
 int attn_run(const void* qkv, const void* scratch, int n_seqs, int64_t T, int nh, int half_window,
-             int bm, void* out, int32_t* status, cudaStream_t st);
+             int bm, void* out, int32_t* status, cudaStream_t st, float* lse = nullptr);
 // Full / banded attention with two CTAs per SM and the accumulator in tensor memory.
 int attn_run_global_tc(const void* qkv, const int4* tile_info, const int32_t* total_tiles,
-                       int64_t max_tiles, int64_t T, int nh, int half_window, void* out,
+                       int64_t max_tiles, int64_t T, int nh, int half_window, void* out, float* lse,
                        int32_t* status, cudaStream_t st);
 // Sliding-window (half window 64) attention with two CTAs per SM, S / P / O in place in tensor memory.
 int attn_run_local_tc2(const void* qkv, const int4* tile_info, const int32_t* total_tiles,
-                       int64_t max_tiles, int64_t T, int nh, void* out, int32_t* status,
+                       int64_t max_tiles, int64_t T, int nh, void* out, float* lse, int32_t* status,
                        cudaStream_t st);
 
 // The final LayerNorm of a forward fused with the pooling head (pool.cu): pooled_out [n_seqs, H] =

@@ -22,6 +22,7 @@ enum StatusCode : int {
   ST_BAD_TOKEN_ID = 301,
   ST_BAD_POSITION = 302,
   ST_BAD_CU_SEQLENS = 303,  // a boundary outside [0, T] or running backwards (clamped, not followed)
+  ST_BAD_TARGET = 304,      // target token outside the vocabulary (treated as ignored)
 };
 
 __device__ __forceinline__ void set_status(int* status, int code) {

@@ -17,7 +17,8 @@
  * 101-103: a bounded wait inside a GEMM ran out; 201-204: inside an attention kernel;
  * 301: token id outside the vocabulary (row 0 was used); 302: position outside the RoPE table
  * (position 0 was used); 303: a cu_seqlens entry outside [0, T] or smaller than its predecessor
- * (clamped into range: no kernel follows a boundary outside the caller's buffers).
+ * (clamped into range: no kernel follows a boundary outside the caller's buffers); 304: target token
+ * outside the vocabulary (its row is treated as ignored).
  *
  * Inputs are expected to be finite.  The attention kernels fetch whole key/value tiles and mask
  * the scores of keys outside a sequence to zero probability, so a NaN or Inf in one sequence's
@@ -44,6 +45,11 @@ extern "C" {
 #define PE_ERR_WORKSPACE (-3)  /* workspace too small */
 #define PE_ERR_DEVICE (-4)     /* a kernel recorded a fault in the status word */
 #define PE_ERR_UNSUPPORTED (-5)/* not an sm_100 device, or shape outside the kernels' envelope */
+
+/* Element types of the entry points that take one. */
+#define PE_BF16 0
+#define PE_FP16 1
+#define PE_FP32 2
 
 /* Per-layer weights, HF ModernBERT layout, all bf16, never copied or re-laid out
  * (packed_encoders/pack.py:3-6).  attn_norm_w is NULL where the layer's attn_norm
@@ -254,6 +260,66 @@ int pe_attn_varlen(const void* qkv, const int32_t* cu_seqlens, int n_seqs, int64
 int pe_attn_varlen_static(const void* qkv, const int32_t* cu_seqlens, int n_seqs, int64_t T,
                           int nh, int half_window, int max_seqlen, void* out, int32_t* status,
                           void* stream);
+
+/* ---- training operators -------------------------------------------------------- */
+
+/* pe_attn_varlen (same arguments, same out) that also stores what a backward pass needs: lse, fp32
+ * [nh, T], the natural logarithm of each query's sum of exp(q k^T / 8).  Rows outside every sequence
+ * (before cu_seqlens[0], at or behind cu_seqlens[n_seqs]) get zeros in out and -inf in lse.  out must
+ * be 16-byte aligned. */
+int pe_attn_varlen_lse(const void* qkv, const int32_t* cu_seqlens, int n_seqs, int64_t T, int nh,
+                       int half_window, int max_seqlen, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Bytes of scratch pe_attn_varlen_backward needs for T tokens and nh heads. */
+size_t pe_attn_backward_workspace_bytes(int64_t T, int nh);
+
+/* Gradient of that attention with respect to qkv (the role of the backward half of the varlen
+ * attention of packed_encoders/ops.py:515-532 under autograd).  dout, out: bf16 [T, nh*64]; qkv as in
+ * the forward (q and k already rotated); lse from the forward; dqkv: bf16 [T, 3*nh*64].  The
+ * probabilities are recomputed; sums are fp32 in a fixed order without atomics, so repeated calls
+ * give the same bits.  Rows outside every sequence get zero gradients.  max_seqlen is not needed.
+ * table and position_ids (both or neither): the rotation table and positions that the forward's q
+ * and k were rotated with; dq and dk are then turned back, i.e. dqkv is the gradient with respect to
+ * the qkv before pe_rope_qk_inplace.  A position outside the table counts as 0 (status 302).  The
+ * values of rows behind the last sequence are never read into another row's gradient. */
+int pe_attn_varlen_backward(const void* dout, const void* qkv, const void* out, const float* lse,
+                            const int32_t* cu_seqlens, int n_seqs, int64_t T, int nh, int half_window,
+                            const int64_t* position_ids, const void* table, int max_positions, void* dqkv,
+                            void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Dropout without a stored mask: y = keep ? x / (1 - p') : 0, plus residual if it is not NULL; fp32
+ * arithmetic, one rounding.  p' is p rounded to a multiple of 2^-16.  keep(e) depends on seed,
+ * position and the element number e alone: field e % 8 (16 bits, low half of word 0 first) of
+ * Philox4x32-10 with counter position + e / 8 and key = seed is at least p' * 65536.  The gradient
+ * with respect to x is therefore the same call on dy.  A call uses (n + 7) / 8 positions.
+ * rng: device int64[2] = {seed, position}, read when the kernel runs, so a captured call sees what the
+ * program has put there since; rng_used (may be NULL): device int64[2] that receives them, for a
+ * backward pass that comes after the program has moved on.  x, residual, y: n elements of type
+ * dtype (PE_BF16, PE_FP16, PE_FP32); y may be x or residual. */
+int pe_dropout(const void* x, const void* residual, int dtype, int64_t n, double p, const int64_t* rng,
+               int64_t* rng_used, void* y, void* stream);
+
+/* Log-probabilities over a vocabulary.  logits: rows of `vocab` elements of type dtype, ld >= vocab
+ * elements apart; targets int64 [rows].  Per row, all fp32: lse = log sum exp(x), lse_rest what the
+ * rounding of lse left (for the backward pass; log p = (x - lse) - lse_rest keeps its precision far
+ * from zero), entropy = -sum p log p, logprobs = x[target] - lse (0 where target == ignore_index); top_ids int64 and
+ * top_logprobs [rows, top_k]: the top_k largest logits in descending order, equal ones by lowest
+ * index, a NaN above everything (both may be NULL with top_k = 0; top_k <= 32).  A logit of -inf has
+ * probability 0; a row with a NaN, a +inf or nothing but -inf gives NaN, as log-softmax does.  A
+ * target outside [0, vocab) that is not ignore_index is reported (status 304) and ignored. */
+int pe_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                      const int64_t* targets, int64_t ignore_index, int top_k, float* logprobs,
+                      float* entropy, float* lse, float* lse_rest, int64_t* top_ids, float* top_logprobs, int32_t* status,
+                      void* stream);
+
+/* Gradient of the above with respect to the logits, from the gradients of logprobs, entropy and lse
+ * (fp32 [rows], each may be NULL): dx_j = g ([j = target] - p_j) - h p_j (log p_j + H) + z p_j.
+ * lse, lse_rest and entropy from the forward.  dlogits: same type, ld_out >= vocab; it may be logits itself. */
+int pe_token_logprobs_backward(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                               const int64_t* targets, int64_t ignore_index, const float* lse,
+                               const float* lse_rest, const float* entropy, const float* d_logprobs,
+                               const float* d_entropy, const float* d_lse, void* dlogits, int64_t ld_out, void* stream);
 
 /* ---- whole forward ---------------------------------------------------------- */
 
