@@ -35,44 +35,64 @@
 
 namespace pe {
 
-constexpr int BW_COMPUTE_WARPS = 8;
-constexpr int BW_THREADS = 32 * (BW_COMPUTE_WARPS + 2);
-constexpr int BW_TILE = 128;
-constexpr int BW_TILE_BYTES = BW_TILE * 64 * 2;  // one 128 x 64 bf16 tile
-constexpr int BW_STAGES = 4;                     // column tiles in flight: (Q, dO) or (K, V)
-constexpr int BW_STATS_BYTES = 2 * BW_TILE * 4;  // lse and delta of 128 columns
+// Three groups of four compute warps take a row tile's column tiles in turn; each is a chain of tensor
+// memory loads, exponentials, stores and barrier round trips that no group could hide alone, and
+// three of them fill each other's gaps.  A column tile is 64 wide so that each group can own the two
+// 64-column buffers it needs beside the accumulators.
+constexpr int BW_GROUPS = 3;
+constexpr int BW_COMPUTE_WARPS = 4 * BW_GROUPS;
+// Beside them a producer warp and two warps that issue MMAs: one thread that waits, issues and commits
+// for all four products of a tile took longer over it than the tensor core.
+constexpr int BW_PRODUCER = BW_COMPUTE_WARPS;
+constexpr int BW_SCORES = BW_COMPUTE_WARPS + 1;      // S and dP
+constexpr int BW_ACCUMULATE = BW_COMPUTE_WARPS + 2;  // dV and dK, or dQ
+constexpr int BW_THREADS = 32 * (BW_COMPUTE_WARPS + 3);
+constexpr int BW_TILE = 128;                        // rows of a row tile
+constexpr int BW_COLS = 64;                         // columns of a column tile
+constexpr int BW_A_BYTES = BW_TILE * 64 * 2;        // one operand of a row tile
+constexpr int BW_B_BYTES = BW_COLS * 64 * 2;        // one operand of a column tile
+constexpr int BW_STAGES = 6;                        // column tiles in flight: (Q, dO) or (K, V)
+constexpr int BW_STATS_BYTES = 2 * BW_COLS * 4;     // lse and delta of a column tile
+constexpr int BW_OUT_BYTES = 32 * 128;              // a warp's 32 rows of one gradient on their way out
 constexpr uint32_t BW_TMEM_COLS = 512;
-constexpr uint32_t BW_S_COL = 0;      // S: two buffers of 128 columns; P in place (bf16 pairs)
-constexpr uint32_t BW_DP_COL = 256;   // dP: 128 columns; dS in place
-constexpr uint32_t BW_ACC1_COL = 384; // dK or dQ
-constexpr uint32_t BW_ACC2_COL = 448; // dV
+// Tensor memory: group w has two buffers of 64 columns at 128 w.  For its i-th tile the scores go to
+// buffer i % 2 and dP to the other.  The scores are replaced in place by P (32 columns of bf16 pairs)
+// and dS (32 more).  Once dP has been read its buffer takes the group's next scores; once P and dS have
+// been multiplied theirs takes the next dP.
+constexpr uint32_t BW_ACC1_COL = 384;  // dK or dQ
+constexpr uint32_t BW_ACC2_COL = 448;  // dV
 
-// Barriers of one pass; each pass has its own set.
+// Barriers of one pass; each pass has its own set.  [w]: one per group, whose phases the group's own
+// tiles (epilogues, for ACC_FULL) count, so that nobody who waits can be two phases behind.
 enum {
-  WB_FULL = 0,        // BW_STAGES
-  WB_EMPTY = 4,       // BW_STAGES
-  WB_A_FULL = 8,      // 2
-  WB_A_EMPTY = 10,    // 2
-  WB_S_FULL = 12,     // 2
-  // 2 (tile parity), one arrival per compute warp: P written (key pass) / S read (query pass).  Two,
-  // because a warp may be done with the scores of tile g + 1 before another is with those of tile g.
-  WB_P_FULL = 14,
-  WB_DP_FULL = 16,
-  WB_DS_FULL = 17,    // one arrival per compute warp
-  WB_DV_DONE = 18,
-  WB_DK_DONE = 19,    // dK (or dQ) of a tile has retired
-  WB_ACC_EMPTY = 20,  // one arrival per compute warp: the item's accumulators have been read
-  WB_COUNT = 21
+  WB_FULL = 0,                           // [stage]
+  WB_EMPTY = WB_FULL + BW_STAGES,        // [stage]
+  WB_A_FULL = WB_EMPTY + BW_STAGES,      // [2]
+  WB_A_EMPTY = WB_A_FULL + 2,            // [2]
+  WB_S_FULL = WB_A_EMPTY + 2,            // [w]
+  WB_DP_FULL = WB_S_FULL + BW_GROUPS,    // [w]
+  WB_DK_DONE = WB_DP_FULL + BW_GROUPS,   // [w] a tile's dK (or dQ) has retired, and its dV before it
+  WB_ACC_FULL = WB_DK_DONE + BW_GROUPS,  // [w] the products of the item whose epilogue is w's have retired
+  // from here on: one arrival per warp of a group
+  // [2 w + parity of the group's tile] P written (key pass).  Two, because a group may reach its next
+  // tile's P before this tile's dV has been issued (but not the one after: that takes this tile's dK).
+  WB_P_FULL = WB_ACC_FULL + BW_GROUPS,
+  WB_DP_READ = WB_P_FULL + 2 * BW_GROUPS,  // [w]
+  WB_DS_FULL = WB_DP_READ + BW_GROUPS,   // [w]
+  WB_ACC_EMPTY = WB_DS_FULL + BW_GROUPS, // the item's accumulators have been read
+  WB_OUT_FREE = WB_ACC_EMPTY + 1,        // the item's gradients have left shared memory
+  WB_COUNT = WB_OUT_FREE + 1
 };
-constexpr int BW_BAR_OFFSET = (4 + 2 * BW_STAGES) * BW_TILE_BYTES + BW_STAGES * BW_STATS_BYTES;
+constexpr int BW_OUT_OFFSET = 4 * BW_A_BYTES + BW_STAGES * 2 * BW_B_BYTES;
+constexpr int BW_STATS_OFFSET = BW_OUT_OFFSET + 8 * BW_OUT_BYTES;
+constexpr int BW_BAR_OFFSET = BW_STATS_OFFSET + BW_STAGES * BW_STATS_BYTES;
 constexpr int BW_SMEM = BW_BAR_OFFSET + 2 * WB_COUNT * 8 + 16;
 
 struct BwArgs {
   const int2* row_range;    // [T]: columns [x, y) that row t attends
   const int2* tile_range;   // [tiles]: their union over a tile of 128 rows
-  const float* lse2;        // [nh, T]: lse * log2(e)
-  const float* delta;       // [nh, T]
-  __nv_bfloat16* dqkv;      // [T, 3 nh 64]
+  const float* neg_lse2;    // [nh, T]: -lse * log2(e)
+  const float* neg_delta;   // [nh, T]
   const int64_t* pos;       // [T] or NULL: rotation of q and k undone on dq and dk
   const __nv_bfloat16* table;
   int max_positions;
@@ -82,14 +102,14 @@ struct BwArgs {
 
 // ---- preparation ------------------------------------------------------------------
 // Grid (tiles, heads), 256 threads.  Every block: delta of its 128 rows and head, eight lanes per
-// row, and lse in the exponent's base.  Blocks of head 0 also find each row's sequence and window.
+// row, and lse in the exponent's base, both negated as the passes use them.  Blocks of head 0 also find each row's sequence and window.
 // Boundaries are not trusted: a row whose sequence does not come out as begin <= t < end within
 // [0, T] attends nothing, and an entry outside [0, T] or below its predecessor is reported.
 __global__ void __launch_bounds__(256)
 attn_bwd_prepare_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ dout,
                         const float* __restrict__ lse, const int32_t* __restrict__ cu_seqlens, int n_seqs,
                         int T, int nh, int half_window, int2* __restrict__ row_range,
-                        int2* __restrict__ tile_range, float* __restrict__ lse2, float* __restrict__ delta,
+                        int2* __restrict__ tile_range, float* __restrict__ neg_lse2, float* __restrict__ neg_delta,
                         int* status) {
   const int tile = blockIdx.x, head = blockIdx.y;
   const int H = nh * 64;
@@ -110,8 +130,8 @@ attn_bwd_prepare_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat
     for (int o = 1; o < 8; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     if (t < T && sub == 0) {
       const int64_t at = int64_t(head) * T + t;
-      delta[at] = acc;
-      lse2[at] = lse[at] * 1.4426950408889634f;
+      neg_delta[at] = -acc;
+      neg_lse2[at] = lse[at] * -1.4426950408889634f;
     }
   }
   if (head != 0) return;
@@ -160,34 +180,46 @@ attn_bwd_prepare_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat
 
 // ---- the two passes -----------------------------------------------------------------
 
-// A cursor over the column tiles of this CTA's items.  Item = (row tile, head), head fastest.
-struct BwCursor {
-  int item, ord;  // item and how many items this CTA began before it
-  int j, n;       // column tile and how many the item has (at least one: an empty item runs one, masked)
-  int lo, hi;     // columns of the row tile
-  __device__ __forceinline__ void open(const BwArgs& a) {
-    if (item >= a.n_items) return;
-    const int2 r = __ldg(a.tile_range + item / a.nh);
-    lo = r.x;
-    hi = r.y;
-    j = 0;
-    n = max((hi - lo + BW_TILE - 1) / BW_TILE, 1);
+// One of this CTA's items: (row tile, head), head fastest, every gridDim-th.  The column range of the
+// item after is fetched a whole item ahead, and nothing is divided on the way.
+struct BwItem {
+  int index, tile, head;
+  int lo, hi;  // columns of the row tile
+  int n;       // its column tiles (at least one: an empty item runs one, masked)
+  int d_tile, d_head;
+  int2 ahead;
+  __device__ __forceinline__ void fetch(const BwArgs& a) {
+    int t = tile + d_tile, h = head + d_head;
+    if (h >= a.nh) ++t;
+    ahead = index + int(gridDim.x) < a.n_items ? __ldg(a.tile_range + t) : make_int2(0, 0);
+  }
+  __device__ __forceinline__ void open(const BwArgs& a, int2 range) {
+    lo = range.x;
+    hi = range.y;
+    n = max((hi - lo + BW_COLS - 1) / BW_COLS, 1);
+    fetch(a);
   }
   __device__ __forceinline__ void start(const BwArgs& a, int first) {
-    item = first;
-    ord = 0;
-    open(a);
+    index = first;
+    tile = first / a.nh;
+    head = first % a.nh;
+    d_tile = int(gridDim.x) / a.nh;
+    d_head = int(gridDim.x) % a.nh;
+    open(a, index < a.n_items ? __ldg(a.tile_range + tile) : make_int2(0, 0));
   }
-  __device__ __forceinline__ bool valid(const BwArgs& a) const { return item < a.n_items; }
-  __device__ __forceinline__ void advance(const BwArgs& a) {
-    if (++j == n) {
-      item += gridDim.x;
-      ++ord;
-      open(a);
+  __device__ __forceinline__ bool valid(const BwArgs& a) const { return index < a.n_items; }
+  __device__ __forceinline__ void next(const BwArgs& a) {
+    index += gridDim.x;
+    tile += d_tile;
+    head += d_head;
+    if (head >= a.nh) {
+      head -= a.nh;
+      ++tile;
     }
+    open(a, ahead);
   }
   // first column of tile j: the last tile ends at hi (it may start below zero: filled, then masked)
-  __device__ __forceinline__ int col0() const { return j + 1 == n ? hi - BW_TILE : lo + j * BW_TILE; }
+  __device__ __forceinline__ int col0(int j) const { return j + 1 == n ? hi - BW_COLS : lo + j * BW_COLS; }
 };
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
@@ -204,332 +236,390 @@ __device__ __forceinline__ float4 lds128(uint32_t addr) {
   return v;
 }
 
-// Stores 64 gradient values of one row as bf16, after undoing the rotation of its position if a
-// table is given (the transpose of the rotation applied to q and k).
-__device__ __forceinline__ void bw_store_row(const BwArgs& a, int t, bool empty, bool rotated, float scale,
-                                             const uint32_t (&lo)[32], const uint32_t (&hi)[32],
-                                             __nv_bfloat16* dst) {
-  const uint4* trow = nullptr;
-  if (rotated) {
-    int64_t p = a.pos[t];
-    if (p < 0 || p >= a.max_positions) {
-      set_status(a.status, ST_BAD_POSITION);
-      p = 0;
-    }
-    trow = reinterpret_cast<const uint4*>(a.table + p * 64);
-  }
+// 64 accumulated values of a row, scaled, as 32 bf16 pairs; with `trow` (the rotation table's row of the
+// row's position) the rotation is undone first: the transpose of what was applied to q and k.
+__device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, const uint4* trow, uint32_t (&out)[32]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    float x[8], y[8];
+  for (int c = 0; c < 2; ++c) {  // dimensions [16 c, 16 c + 16) and those they are paired with, 32 further on
+    uint32_t lo[16], hi[16];
+    g_tmem_ld16(acc_addr + c * 16, lo);
+    g_tmem_ld16(acc_addr + 32 + c * 16, hi);
+    tmem_ld_wait();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = __uint_as_float(lo[c * 8 + e]) * scale;
-      y[e] = __uint_as_float(hi[c * 8 + e]) * scale;
-    }
-    if (rotated) {
-      float cs[8], sn[8];
-      unpack8(__ldg(trow + c), cs);
-      unpack8(__ldg(trow + 4 + c), sn);
+    for (int h = 0; h < 2; ++h) {
+      float x[8], y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float u = x[e], w = y[e];
-        x[e] = fmaf(u, cs[e], w * sn[e]);
-        y[e] = fmaf(w, cs[e], -(u * sn[e]));
+        x[e] = __uint_as_float(lo[h * 8 + e]) * scale;
+        y[e] = __uint_as_float(hi[h * 8 + e]) * scale;
+      }
+      if (trow != nullptr) {
+        float cs[8], sn[8];
+        unpack8(__ldg(trow + c * 2 + h), cs);
+        unpack8(__ldg(trow + 4 + c * 2 + h), sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float u = x[e], w = y[e];
+          x[e] = fmaf(u, cs[e], w * sn[e]);
+          y[e] = fmaf(w, cs[e], -(u * sn[e]));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        out[c * 8 + h * 4 + e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+        out[16 + c * 8 + h * 4 + e] = pack_bf16(y[2 * e], y[2 * e + 1]);
       }
     }
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    *reinterpret_cast<uint4*>(dst + c * 8) = empty ? zero : pack8(x);
-    *reinterpret_cast<uint4*>(dst + 32 + c * 8) = empty ? zero : pack8(y);
   }
 }
+// Puts a row's 64 bf16 values (zeros if it is empty) into the warp's 128-byte-swizzled staging block.
+__device__ __forceinline__ void bw_stage_row(uint32_t block, int lane, const uint32_t (&v)[32], bool empty) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(block + lane * 128 + ((i ^ (lane & 7)) << 4)),
+                 "r"(empty ? 0u : v[4 * i]), "r"(empty ? 0u : v[4 * i + 1]), "r"(empty ? 0u : v[4 * i + 2]),
+                 "r"(empty ? 0u : v[4 * i + 3])
+                 : "memory");
+}
+
+struct BwMaps {  // rows x 64 columns: row tiles (128), column tiles (64), a warp's rows of the result (32)
+  CUtensorMap qkv, qkv_cols, dout, dout_cols, dqkv;
+};
 
 // KEYS: the key pass (rows are keys, columns are queries), else the query pass.  `first` is this
 // CTA's first item.  Returns false if a bounded wait gave up.
 template <bool KEYS>
-__device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtensorMap& tm_dout, const BwArgs& a,
-                                        int first, uint32_t base, uint32_t bar_base, uint32_t tmem_base) {
+__device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int first, uint32_t base,
+                                        uint32_t bar_base, uint32_t tmem_base) {
   auto bar = [&](int i) { return bar_base + 8u * i; };
-  const uint32_t sA = base;                                // A[buffer]: (K, V) or (Q, dO)
-  const uint32_t sB = base + 4 * BW_TILE_BYTES;            // B[stage]: (Q, dO) or (K, V)
-  const uint32_t sStats = sB + 2 * BW_STAGES * BW_TILE_BYTES;
+  const uint32_t sA = base;                  // A[buffer]: (K, V) or (Q, dO)
+  const uint32_t sB = base + 4 * BW_A_BYTES; // B[stage]: (Q, dO) or (K, V)
+  const uint32_t sStats = base + BW_STATS_OFFSET;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int H = a.nh * 64;
   int* status = a.status;
   bool ok = true;
+  BwItem it;
+  it.start(a, first);
 
-  if (warp == BW_COMPUTE_WARPS) {
+  if (warp == BW_PRODUCER) {
     // ---------------------------------------------------------------- producer
-    BwCursor c;
-    c.start(a, first);
-    uint32_t g = 0;
-    while (c.valid(a)) {
-      const int row0 = (c.item / a.nh) * BW_TILE, head = c.item % a.nh;
-      if (c.j == 0) {
-        const uint32_t ab = c.ord & 1;
-        if (!mbar_wait(bar(WB_A_EMPTY + ab), ((c.ord >> 1) & 1) ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
-        if (lane == 0) {
-          const uint32_t dst = sA + ab * 2 * BW_TILE_BYTES;
-          mbar_expect_tx(bar(WB_A_FULL + ab), 2 * BW_TILE_BYTES);
-          tma_load_2d(dst, &tm_qkv, bar(WB_A_FULL + ab), (KEYS ? H : 0) + head * 64, row0);
-          if (KEYS) tma_load_2d(dst + BW_TILE_BYTES, &tm_qkv, bar(WB_A_FULL + ab), 2 * H + head * 64, row0);
-          else tma_load_2d(dst + BW_TILE_BYTES, &tm_dout, bar(WB_A_FULL + ab), head * 64, row0);
-        }
-        __syncwarp();
-      }
-      const uint32_t st = g % BW_STAGES;
-      if (!mbar_wait(bar(WB_EMPTY + st), ((g / BW_STAGES) & 1) ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
-      const int col0 = c.col0();
-      if (KEYS) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int q = min(max(col0 + i * 32 + lane, 0), a.T - 1);
-          const int64_t at = int64_t(head) * a.T + q;
-          const uint32_t dst = sStats + st * BW_STATS_BYTES + (i * 32 + lane) * 4;
-          cp_async4(dst, a.lse2 + at);
-          cp_async4(dst + BW_TILE * 4, a.delta + at);
-        }
-        cp_async_arrive(bar(WB_FULL + st));
-      }
+    uint32_t st = 0, phase = 0, loads = 0, ord = 0;
+    for (; it.valid(a) && ok; it.next(a), ++ord) {
+      const uint32_t ab = ord & 1;
+      const int c = it.head * 64, row0 = it.tile * BW_TILE;
+      if (!mbar_wait(bar(WB_A_EMPTY + ab), ((ord >> 1) & 1) ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
       if (lane == 0) {
-        const uint32_t dst = sB + st * 2 * BW_TILE_BYTES;
-        mbar_expect_tx(bar(WB_FULL + st), 2 * BW_TILE_BYTES);
-        tma_load_2d(dst, &tm_qkv, bar(WB_FULL + st), (KEYS ? 0 : H) + head * 64, col0);
-        if (KEYS) tma_load_2d(dst + BW_TILE_BYTES, &tm_dout, bar(WB_FULL + st), head * 64, col0);
-        else tma_load_2d(dst + BW_TILE_BYTES, &tm_qkv, bar(WB_FULL + st), 2 * H + head * 64, col0);
+        const uint32_t dst = sA + ab * 2 * BW_A_BYTES;
+        mbar_expect_tx(bar(WB_A_FULL + ab), 2 * BW_A_BYTES);
+        tma_load_2d(dst, &m.qkv, bar(WB_A_FULL + ab), (KEYS ? H : 0) + c, row0);
+        if (KEYS) tma_load_2d(dst + BW_A_BYTES, &m.qkv, bar(WB_A_FULL + ab), 2 * H + c, row0);
+        else tma_load_2d(dst + BW_A_BYTES, &m.dout, bar(WB_A_FULL + ab), c, row0);
       }
       __syncwarp();
-      ++g;
-      c.advance(a);
+      const float* lse_head = a.neg_lse2 + int64_t(it.head) * a.T;
+      const float* delta_head = a.neg_delta + int64_t(it.head) * a.T;
+      for (int j = 0; j < it.n; ++j) {
+        if (!mbar_wait(bar(WB_EMPTY + st), phase ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
+        const int col0 = it.col0(j);
+        if (KEYS) {
+#pragma unroll
+          for (int i = 0; i < BW_COLS / 32; ++i) {
+            const int q = min(max(col0 + i * 32 + lane, 0), a.T - 1);
+            const uint32_t dst = sStats + st * BW_STATS_BYTES + (i * 32 + lane) * 4;
+            cp_async4(dst, lse_head + q);
+            cp_async4(dst + BW_COLS * 4, delta_head + q);
+          }
+          cp_async_arrive(bar(WB_FULL + st));
+        }
+        if (lane == 0) {
+          const uint32_t dst = sB + st * 2 * BW_B_BYTES;
+          mbar_expect_tx(bar(WB_FULL + st), 2 * BW_B_BYTES);
+          tma_load_2d(dst, &m.qkv_cols, bar(WB_FULL + st), (KEYS ? 0 : H) + c, col0);
+          if (KEYS) tma_load_2d(dst + BW_B_BYTES, &m.dout_cols, bar(WB_FULL + st), c, col0);
+          else tma_load_2d(dst + BW_B_BYTES, &m.qkv_cols, bar(WB_FULL + st), 2 * H + c, col0);
+        }
+        __syncwarp();
+        ++loads;
+        if (++st == BW_STAGES) {
+          st = 0;
+          phase ^= 1u;
+        }
+      }
     }
     if (!ok) {  // gave up: this CTA's copies must have landed before it can leave
-      for (uint32_t u = g > BW_STAGES ? g - BW_STAGES : 0; u < g; ++u)
+      for (uint32_t u = loads > BW_STAGES ? loads - BW_STAGES : 0; u < loads; ++u)
         mbar_wait(bar(WB_FULL + u % BW_STAGES), (u / BW_STAGES) & 1, status, ST_ATTN_TIMEOUT);
-      if (c.ord > 0) mbar_wait(bar(WB_A_FULL + ((c.ord - 1) & 1)), ((c.ord - 1) >> 1) & 1, status, ST_ATTN_TIMEOUT);
+      for (uint32_t u = ord > 1 ? ord - 2 : 0; u <= ord; ++u)  // (one that was never issued runs into its limit)
+        mbar_wait(bar(WB_A_FULL + (u & 1)), (u >> 1) & 1, status, ST_ATTN_TIMEOUT);
     }
-  } else if (warp == BW_COMPUTE_WARPS + 1) {
-    // ---------------------------------------------------------------- MMA issuer
+  } else if (warp == BW_SCORES) {
+    // ---------------------------------------------------------------- S and dP
     if (elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, 0);
-      constexpr uint32_t idesc_acc = umma_idesc_bf16(128, 64, 1);  // B is MN-major: its rows are the contraction
-      BwCursor sc, dc, mc;  // scores, dP, accumulation
-      sc.start(a, first);
-      dc = sc;
-      mc = sc;
-      uint32_t gs = 0, gd = 0, g = 0;
+      constexpr uint32_t idesc = umma_idesc_bf16(BW_TILE, BW_COLS, 0);
       auto wait = [&](int b, uint32_t parity) {
-        if (ok && !mbar_wait(bar(b), parity, status, ST_ATTN_MMA_TIMEOUT)) ok = false;
+        if (!mbar_wait(bar(b), parity, status, ST_ATTN_MMA_TIMEOUT)) ok = false;
         return ok;
       };
-      auto scores = [&](uint32_t d_col, uint32_t a_tile, uint32_t b_tile) {
-        const uint64_t ad = umma_smem_desc_sw128(a_tile, 1024), bd = umma_smem_desc_sw128(b_tile, 1024);
+      auto product = [&](uint32_t d_col, uint64_t ad, uint64_t bd) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_ss(tmem_base + d_col, ad + 2u * kk, bd + 2u * kk, idesc_s, kk != 0 ? 1u : 0u);
+          umma_ss(tmem_base + d_col, ad + 2u * kk, bd + 2u * kk, idesc, kk != 0 ? 1u : 0u);
       };
-      // acc += X B, X (bf16 pairs of 128 columns) in tensor memory: the two halves of a tile were
-      // written by different warps, each in place over its own 64 fp32 columns
-      auto accumulate = [&](uint32_t acc_col, uint32_t x_col, uint32_t b_tile, bool first_tile) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          g_umma_ts(tmem_base + acc_col, tmem_base + x_col + (kk >> 2) * 64 + (kk & 3) * 8,
-                    umma_smem_desc_sw128(b_tile + kk * 2048, 1024), idesc_acc, (!first_tile || kk != 0) ? 1u : 0u);
-      };
-      auto issue_s = [&]() {
-        const uint32_t st = gs % BW_STAGES;
-        if (sc.j == 0 && !wait(WB_A_FULL + (sc.ord & 1), (sc.ord >> 1) & 1)) return;
-        if (!wait(WB_FULL + st, (gs / BW_STAGES) & 1)) return;
-        tc_fence_after();
-        scores(BW_S_COL + (gs & 1) * 128, sA + (sc.ord & 1) * 2 * BW_TILE_BYTES, sB + st * 2 * BW_TILE_BYTES);
-        umma_commit(bar(WB_S_FULL + (gs & 1)));
-        ++gs;
-        sc.advance(a);
-      };
-      auto issue_dp = [&]() {  // its operands arrived with those of the scores of the same tile
-        const uint32_t st = gd % BW_STAGES;
-        scores(BW_DP_COL, sA + ((dc.ord & 1) * 2 + 1) * BW_TILE_BYTES, sB + (st * 2 + 1) * BW_TILE_BYTES);
-        umma_commit(bar(WB_DP_FULL));
-        if (dc.j + 1 == dc.n) umma_commit(bar(WB_A_EMPTY + (dc.ord & 1)));
-        ++gd;
-        dc.advance(a);
-      };
-      if (sc.valid(a)) {
-        issue_s();
-        if (ok) issue_dp();
-        if (ok && sc.valid(a)) issue_s();
+      // group, its tile's parity, stage and its phase of the tile about to be issued
+      uint32_t w = 0, i = 0, st = 0, phase = 0, ord = 0;
+      for (; it.valid(a) && ok; it.next(a), ++ord) {
+        const uint64_t a1 = umma_smem_desc_sw128(sA + (ord & 1) * 2 * BW_A_BYTES, 1024);
+        const uint64_t a2 = umma_smem_desc_sw128(sA + ((ord & 1) * 2 + 1) * BW_A_BYTES, 1024);
+        if (!wait(WB_A_FULL + (ord & 1), (ord >> 1) & 1)) break;
+        for (int j = 0; j < it.n; ++j) {
+          const uint64_t b1 = umma_smem_desc_sw128(sB + st * 2 * BW_B_BYTES, 1024);
+          const uint32_t s_col = w * 128 + (i & 1) * 64;
+          if (!wait(WB_FULL + st, phase)) break;
+          // the group's last dP has been read: its buffer takes these scores
+          if (i > 0 && !wait(WB_DP_READ + w, (i & 1) ^ 1u)) break;
+          tc_fence_after();
+          product(s_col, a1, b1);
+          umma_commit(bar(WB_S_FULL + w));
+          // the group's last P and dS have been multiplied: their buffer takes this dP
+          if (i > 0 && !wait(WB_DK_DONE + w, (i & 1) ^ 1u)) break;
+          tc_fence_after();
+          product(s_col ^ 64u, a2, b1 + (BW_B_BYTES >> 4));
+          umma_commit(bar(WB_DP_FULL + w));
+          if (++w == BW_GROUPS) {
+            w = 0;
+            ++i;
+          }
+          if (++st == BW_STAGES) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) umma_commit(bar(WB_A_EMPTY + (ord & 1)));
       }
-      while (ok && mc.valid(a)) {
-        const uint32_t st = g % BW_STAGES;
-        const uint32_t b1 = sB + st * 2 * BW_TILE_BYTES, b2 = b1 + BW_TILE_BYTES;
-        if (!wait(WB_P_FULL + (g & 1), (g >> 1) & 1)) break;
+    }
+    __syncwarp();
+    ok = __all_sync(0xffffffffu, ok);
+  } else if (warp == BW_ACCUMULATE) {
+    // ---------------------------------------------------------------- dV and dK, or dQ
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_bf16(BW_TILE, 64, 1);  // B is MN-major: its rows are the contraction
+      auto wait = [&](int b, uint32_t parity) {
+        if (!mbar_wait(bar(b), parity, status, ST_ATTN_MMA_TIMEOUT)) ok = false;
+        return ok;
+      };
+      // acc += X B, X (bf16 pairs of 64 columns) in tensor memory
+      auto accumulate = [&](uint32_t acc_col, uint32_t x_col, uint64_t bd, bool first_tile) {
+#pragma unroll
+        for (int kk = 0; kk < BW_COLS / 16; ++kk)
+          g_umma_ts(tmem_base + acc_col, tmem_base + x_col + kk * 8, bd + uint32_t(kk * 2048 >> 4), idesc,
+                    (!first_tile || kk != 0) ? 1u : 0u);
+      };
+      uint32_t w = 0, i = 0, st = 0, phase = 0, ord = 0;
+      for (; it.valid(a) && ok; it.next(a), ++ord) {
         // the previous item's accumulators must have been read before they are overwritten
-        if (mc.j == 0 && mc.ord > 0 && !wait(WB_ACC_EMPTY, (mc.ord - 1) & 1)) break;
-        tc_fence_after();
-        if (KEYS) {
-          accumulate(BW_ACC2_COL, BW_S_COL + (g & 1) * 128, b2, mc.j == 0);  // dV += P^T dO
-          umma_commit(bar(WB_DV_DONE));
-        } else if (sc.valid(a)) {
-          issue_s();  // the scores of tile g are in registers: its buffer takes those of tile g + 2
+        if (ord > 0 && !wait(WB_ACC_EMPTY, (ord & 1) ^ 1u)) break;
+        for (int j = 0; j < it.n; ++j) {
+          const uint64_t b1 = umma_smem_desc_sw128(sB + st * 2 * BW_B_BYTES, 1024);
+          const uint32_t s_col = w * 128 + (i & 1) * 64;
+          if (!wait(WB_FULL + st, phase)) break;
+          if (KEYS) {
+            if (!wait(WB_P_FULL + 2 * w + (i & 1), (i >> 1) & 1)) break;
+            tc_fence_after();
+            accumulate(BW_ACC2_COL, s_col, b1 + (BW_B_BYTES >> 4), j == 0);  // dV += P^T dO
+          }
+          if (!wait(WB_DS_FULL + w, i & 1)) break;
+          tc_fence_after();
+          accumulate(BW_ACC1_COL, s_col + 32, b1, j == 0);  // dK += dS^T Q, dQ += dS K
+          umma_commit(bar(WB_DK_DONE + w));
+          umma_commit(bar(WB_EMPTY + st));
+          if (j + 1 == it.n) umma_commit(bar(WB_ACC_FULL + w));
+          if (++w == BW_GROUPS) {
+            w = 0;
+            ++i;
+          }
+          if (++st == BW_STAGES) {
+            st = 0;
+            phase ^= 1u;
+          }
         }
-        if (!wait(WB_DS_FULL, g & 1)) break;
-        tc_fence_after();
-        accumulate(BW_ACC1_COL, BW_DP_COL, b1, mc.j == 0);  // dK += dS^T Q, dQ += dS K
-        umma_commit(bar(WB_EMPTY + st));
-        umma_commit(bar(WB_DK_DONE));
-        if (KEYS && sc.valid(a)) {
-          if (!wait(WB_DV_DONE, g & 1)) break;  // P of tile g has been read: its buffer is free
-          issue_s();
-        }
-        if (ok && dc.valid(a)) {
-          if (!wait(WB_DK_DONE, g & 1)) break;  // dS of tile g has been read
-          issue_dp();
-        }
-        ++g;
-        mc.advance(a);
       }
     }
     __syncwarp();
     ok = __all_sync(0xffffffffu, ok);
   } else {
     // ---------------------------------------------------------------- compute warps
-    const int half = warp >> 2;                      // which 64 columns of a tile
+    const int w = warp >> 2;                         // group
     const int row = (warp & 3) * 32 + lane;          // row of the tile = tensor-memory lane
     const uint32_t lane_addr = tmem_base + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t out_block = base + BW_OUT_OFFSET + (warp & 3) * 2 * BW_OUT_BYTES;
     const float scale_log2 = 0.125f * 1.4426950408889634f;  // 1/sqrt(64) * log2(e)
+    const float2 scale2 = make_float2(scale_log2, scale_log2);
     // After a bounded wait has given up the loops still run to their end, without waiting, so that
     // every thread reaches the common exit.
     auto wait = [&](int b, uint32_t parity) {
       if (ok && !mbar_wait(bar(b), parity, status, ST_ATTN_SOFTMAX_TIMEOUT)) ok = false;
     };
-    BwCursor c;
-    c.start(a, first);
-    uint32_t g = 0;
-    while (c.valid(a)) {
-      const int head = c.item % a.nh;
-      const int t = (c.item / a.nh) * BW_TILE + row;
-      int2 range = make_int2(0, 0);
-      float lse_row = 0.f, delta_row = 0.f;
-      if (t < a.T) {
-        range = __ldg(a.row_range + t);
-        if (!KEYS) {
-          lse_row = __ldg(a.lse2 + int64_t(head) * a.T + t);
-          delta_row = __ldg(a.delta + int64_t(head) * a.T + t);
-        }
-      }
-      const int n = c.n;
-      for (int j = 0; j < n; ++j, ++g) {
-        const uint32_t st = g % BW_STAGES;
-        const uint32_t s_addr = lane_addr + BW_S_COL + (g & 1) * 128 + half * 64;
-        const uint32_t dp_addr = lane_addr + BW_DP_COL + half * 64;
-        const uint32_t stats = sStats + st * BW_STATS_BYTES + half * 256;
-        // valid columns of this row within its 64: [c_lo, c_hi)
-        const int x0 = c.col0() + half * 64;
-        const int c_lo = max(range.x, c.lo + j * BW_TILE) - x0, c_hi = range.y - x0;
-        const bool full = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= 64);
-        if (KEYS) wait(WB_FULL + st, (g / BW_STAGES) & 1);  // lse and delta of the columns
-        wait(WB_S_FULL + (g & 1), (g >> 1) & 1);
-        tc_fence_after();
-        uint32_t p[64];
-        g_tmem_ld32(s_addr, p);
-        g_tmem_ld32(s_addr + 32, p + 32);
-        tmem_ld_wait();
-        if (!KEYS) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(WB_P_FULL + (g & 1)));
-        }
-        const float2 scale2 = make_float2(scale_log2, scale_log2);
-#pragma unroll
-        for (int e = 0; e < 64; e += 4) {
-          float4 l;
-          if (KEYS) l = lds128(stats + e * 4);
-          else l = make_float4(lse_row, lse_row, lse_row, lse_row);
-          const float2 u = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), scale2,
-                                      make_float2(-l.x, -l.y));
-          const float2 w = __ffma2_rn(make_float2(__uint_as_float(p[e + 2]), __uint_as_float(p[e + 3])), scale2,
-                                      make_float2(-l.z, -l.w));
-          p[e] = __float_as_uint(g_ex2(u.x));
-          p[e + 1] = __float_as_uint(g_ex2(u.y));
-          p[e + 2] = __float_as_uint(g_ex2(w.x));
-          p[e + 3] = __float_as_uint(g_ex2(w.y));
-        }
-        if (!full) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) p[e] = (e >= c_lo && e < c_hi) ? p[e] : 0u;
-        }
-        if (KEYS) {  // P^T back in place, as the A operand of dV += P^T dO
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              pk[e] = pack_bf16(__uint_as_float(p[h * 32 + 2 * e]), __uint_as_float(p[h * 32 + 2 * e + 1]));
-            g_tmem_st16(s_addr + h * 16, pk);
-          }
-          g_tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(WB_P_FULL + (g & 1)));
-        }
-        wait(WB_DP_FULL, g & 1);
-        tc_fence_after();
-        uint32_t dp[64];
-        g_tmem_ld32(dp_addr, dp);
-        g_tmem_ld32(dp_addr + 32, dp + 32);
-        tmem_ld_wait();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float4 dl;
-            if (KEYS) dl = lds128(stats + BW_TILE * 4 + (h * 32 + e) * 4);
-            else dl = make_float4(delta_row, delta_row, delta_row, delta_row);
-            const uint32_t* d = dp + h * 32 + e;
-            const uint32_t* q = p + h * 32 + e;
-            const float2 u = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[0]), __uint_as_float(d[1])),
-                                                   make_float2(-dl.x, -dl.y)),
-                                        make_float2(__uint_as_float(q[0]), __uint_as_float(q[1])));
-            const float2 w = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[2]), __uint_as_float(d[3])),
-                                                   make_float2(-dl.z, -dl.w)),
-                                        make_float2(__uint_as_float(q[2]), __uint_as_float(q[3])));
-            pk[e / 2] = pack_bf16(u.x, u.y);
-            pk[e / 2 + 1] = pack_bf16(w.x, w.y);
-          }
-          g_tmem_st16(dp_addr + h * 16, pk);
-        }
-        g_tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(WB_DS_FULL));
-        c.advance(a);
-      }
-      // The item's accumulators.  Key pass: warps 0..3 store dV, warps 4..7 dK.  Query pass: warps
-      // 0..3 store dQ.  Rows that attend nothing are exact zeros.
-      wait(WB_DK_DONE, (g - 1) & 1);
-      tc_fence_after();
-      uint32_t lo[32], hi[32];
-      const bool mine = KEYS || half == 0;
-      const bool is_v = KEYS && half == 0;
-      if (mine) {
-        const uint32_t acc = lane_addr + (is_v ? BW_ACC2_COL : BW_ACC1_COL);
-        g_tmem_ld32(acc, lo);
-        g_tmem_ld32(acc + 32, hi);
-        tmem_ld_wait();
-      }
+    auto arrive = [&](int b) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(WB_ACC_EMPTY));
-      if (mine && ok && t < a.T)
-        bw_store_row(a, t, range.x >= range.y, a.pos != nullptr && !is_v, is_v ? 1.0f : 0.125f, lo, hi,
-                     a.dqkv + int64_t(t) * 3 * H + (KEYS ? (is_v ? 2 * H : H) : 0) + head * 64);
+      if (lane == 0) mbar_arrive(bar(b));
+    };
+    int j = w;                                 // this group's next tile, counted from the item's first
+    uint32_t i = 0, epilogues = 0, ord = 0;    // tiles and epilogues of this group, items so far
+    uint32_t st = w;                           // stage of tile j and how often its ring has gone round
+    uint32_t round = 0;
+    for (; it.valid(a); it.next(a), ++ord) {
+      if (j < it.n) {
+        // what this thread's row brings along
+        const int t = it.tile * BW_TILE + row;
+        int2 range = make_int2(0, 0);
+        float neg_lse = 0.f, neg_delta = 0.f;
+        if (t < a.T) {
+          range = __ldg(a.row_range + t);
+          if (!KEYS) {
+            const int64_t at = int64_t(it.head) * a.T + t;
+            neg_lse = __ldg(a.neg_lse2 + at);
+            neg_delta = __ldg(a.neg_delta + at);
+          }
+        }
+        for (; j < it.n; j += BW_GROUPS, ++i) {
+          const uint32_t s_addr = lane_addr + w * 128 + (i & 1) * 64;
+          const uint32_t dp_addr = s_addr ^ 64u;
+          const uint32_t stats = sStats + st * BW_STATS_BYTES;
+          // valid columns of this row within the tile: [c_lo, c_hi)
+          const int x0 = it.col0(j);
+          const int c_lo = max(range.x, it.lo + j * BW_COLS) - x0, c_hi = range.y - x0;
+          const bool full = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= BW_COLS);
+          wait(WB_S_FULL + w, i & 1);
+          if (KEYS) wait(WB_FULL + st, round & 1);  // complete by now: makes lse and delta visible
+          tc_fence_after();
+          uint32_t p[64];
+          g_tmem_ld32(s_addr, p);
+          tmem_ld_wait();
+          g_tmem_ld32(s_addr + 32, p + 32);  // in flight during the first half's exponentials
+          auto exponentials = [&](int e0) {
+#pragma unroll
+            for (int e = e0; e < e0 + 32; e += 4) {
+              float4 l;
+              if (KEYS) l = lds128(stats + e * 4);
+              else l = make_float4(neg_lse, neg_lse, neg_lse, neg_lse);
+              const float2 u = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), scale2,
+                                          make_float2(l.x, l.y));
+              const float2 v = __ffma2_rn(make_float2(__uint_as_float(p[e + 2]), __uint_as_float(p[e + 3])), scale2,
+                                          make_float2(l.z, l.w));
+              p[e] = __float_as_uint(g_ex2(u.x));
+              p[e + 1] = __float_as_uint(g_ex2(u.y));
+              p[e + 2] = __float_as_uint(g_ex2(v.x));
+              p[e + 3] = __float_as_uint(g_ex2(v.y));
+            }
+          };
+          exponentials(0);
+          tmem_ld_wait();
+          exponentials(32);
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < BW_COLS; ++e) p[e] = (e >= c_lo && e < c_hi) ? p[e] : 0u;
+          }
+          if (KEYS) {  // P^T in place of the first half of the scores: the A operand of dV += P^T dO
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                pk[e] = pack_bf16(__uint_as_float(p[h * 32 + 2 * e]), __uint_as_float(p[h * 32 + 2 * e + 1]));
+              g_tmem_st16(s_addr + h * 16, pk);
+            }
+            g_tmem_st_wait();
+            arrive(WB_P_FULL + 2 * w + (i & 1));
+          }
+          wait(WB_DP_FULL + w, i & 1);
+          tc_fence_after();
+          uint32_t dp[2][16];
+          g_tmem_ld16(dp_addr, dp[0]);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            tmem_ld_wait();
+            if (h < 3) g_tmem_ld16(dp_addr + (h + 1) * 16, dp[(h + 1) & 1]);  // in flight during this quarter
+            else arrive(WB_DP_READ + w);
+            const uint32_t* d = dp[h & 1];
+            uint32_t pk[8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              float4 dl;
+              if (KEYS) dl = lds128(stats + BW_COLS * 4 + (h * 16 + e) * 4);
+              else dl = make_float4(neg_delta, neg_delta, neg_delta, neg_delta);
+              const uint32_t* q = p + h * 16 + e;
+              const float2 u = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])),
+                                                     make_float2(dl.x, dl.y)),
+                                          make_float2(__uint_as_float(q[0]), __uint_as_float(q[1])));
+              const float2 v = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])),
+                                                     make_float2(dl.z, dl.w)),
+                                          make_float2(__uint_as_float(q[2]), __uint_as_float(q[3])));
+              pk[e / 2] = pack_bf16(u.x, u.y);
+              pk[e / 2 + 1] = pack_bf16(v.x, v.y);
+            }
+            g_tmem_st8(s_addr + 32 + h * 8, pk);  // dS in place of the second half
+          }
+          g_tmem_st_wait();
+          arrive(WB_DS_FULL + w);
+          st += BW_GROUPS;
+          if (st >= BW_STAGES) {
+            st -= BW_STAGES;
+            ++round;
+          }
+          if (j + 1 == it.n) {
+            // The group of an item's last tile stores its gradients while the others go on; the row's 64
+            // (or twice 64) values are in registers before the accumulators are handed back.  Rows
+            // that attend nothing are exact zeros; rows beyond T are clipped by the store.
+            const uint4* trow = nullptr;
+            if (a.pos != nullptr && t < a.T) {
+              int64_t ps = a.pos[t];
+              if (ps < 0 || ps >= a.max_positions) {
+                set_status(status, ST_BAD_POSITION);
+                ps = 0;
+              }
+              trow = reinterpret_cast<const uint4*>(a.table + ps * 64);
+            }
+            wait(WB_ACC_FULL + w, epilogues & 1);
+            ++epilogues;
+            tc_fence_after();
+            uint32_t v1[32], v2[32];
+            bw_finish_row(lane_addr + BW_ACC1_COL, 0.125f, trow, v1);
+            if (KEYS) bw_finish_row(lane_addr + BW_ACC2_COL, 1.0f, nullptr, v2);
+            // The staging blocks are shared by the groups.  (Waited for before the accumulators are handed
+            // back, so that the group of the next item finds at most this item's phase pending.)
+            if (ord > 0) wait(WB_OUT_FREE, (ord & 1) ^ 1u);
+            arrive(WB_ACC_EMPTY);
+            const bool empty = range.x >= range.y;
+            bw_stage_row(out_block, lane, v1, empty);
+            if (KEYS) bw_stage_row(out_block + BW_OUT_BYTES, lane, v2, empty);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              const int row0 = it.tile * BW_TILE + (warp & 3) * 32;
+              if (ok && row0 < a.T) {
+                tma_store_2d(&m.dqkv, out_block, (KEYS ? H : 0) + it.head * 64, row0);
+                if (KEYS) tma_store_2d(&m.dqkv, out_block + BW_OUT_BYTES, 2 * H + it.head * 64, row0);
+                tma_store_commit();
+                tma_store_wait_read<0>();
+              }
+              mbar_arrive(bar(WB_OUT_FREE));
+            }
+            __syncwarp();
+          }
+        }
+      }
+      j -= it.n;
     }
+    if (lane == 0) tma_store_wait_all<0>();  // staging memory must outlive the stores that read it
+    __syncwarp();
   }
   return ok;
 }
 
 __global__ void __launch_bounds__(BW_THREADS, 1)
-attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_dout,
-                const BwArgs a) {
+attn_bwd_kernel(const __grid_constant__ BwMaps m, const BwArgs a) {
   extern __shared__ __align__(1024) uint8_t bw_smem[];
   const uint32_t base = smem_u32(bw_smem);
   if (base & 1023u) {  // the swizzled tiles need it; nothing has been allocated yet
@@ -546,15 +636,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
         uint32_t count = 1;
         // stages of the key pass: the TMA issue and 32 lanes' copies of lse and delta
         if (pass == 0 && i >= WB_FULL && i < WB_FULL + BW_STAGES) count = 33;
-        if (i == WB_P_FULL || i == WB_P_FULL + 1 || i == WB_DS_FULL || i == WB_ACC_EMPTY) count = BW_COMPUTE_WARPS;
+        if (i >= WB_P_FULL) count = 4;
         mbar_init(bb + 8u * i, count);
       }
     }
     mbar_fence_init();
-    tma_prefetch_desc(&tm_qkv);
-    tma_prefetch_desc(&tm_dout);
+    tma_prefetch_desc(&m.qkv);
+    tma_prefetch_desc(&m.qkv_cols);
+    tma_prefetch_desc(&m.dout);
+    tma_prefetch_desc(&m.dout_cols);
+    tma_prefetch_desc(&m.dqkv);
   }
-  if (warp == BW_COMPUTE_WARPS + 1) {
+  if (warp == BW_ACCUMULATE) {
     tmem_alloc(tmem_slot, BW_TMEM_COLS);
     tmem_relinquish();
   }
@@ -566,18 +659,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
 
   // Items of both passes form one list, the key pass first; a CTA takes every gridDim-th of it, so
   // the passes need no launch boundary and a small batch runs both at the same time.
-  const bool ok = bw_pass<true>(tm_qkv, tm_dout, a, blockIdx.x, base, bar_base, tmem_base);
+  const bool ok = bw_pass<true>(m, a, blockIdx.x, base, bar_base, tmem_base);
   tc_fence_before();
   const int failed = __syncthreads_or(!ok);
   tc_fence_after();
   if (!failed) {
     int first = int(blockIdx.x) - a.n_items % int(gridDim.x);
     if (first < 0) first += gridDim.x;
-    bw_pass<false>(tm_qkv, tm_dout, a, first, base, bar_base + WB_COUNT * 8, tmem_base);
+    bw_pass<false>(m, a, first, base, bar_base + WB_COUNT * 8, tmem_base);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == BW_COMPUTE_WARPS + 1) {
+  if (warp == BW_ACCUMULATE) {
     tc_fence_after();
     tmem_dealloc(tmem_base, BW_TMEM_COLS);
   }
@@ -636,19 +729,21 @@ extern "C" int pe_attn_varlen_backward(const void* dout, const void* qkv, const 
   if (T == 0) return PE_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  CUtensorMap tm_qkv, tm_dout;
-  int rc = make_tmap_bf16_2d(&tm_qkv, qkv, (uint64_t)T, (uint64_t)nh * 192, (uint64_t)nh * 192, BW_TILE);
-  if (rc != PE_OK) return rc;
-  rc = make_tmap_bf16_2d(&tm_dout, dout, (uint64_t)T, (uint64_t)nh * 64, (uint64_t)nh * 64, BW_TILE);
+  BwMaps m;
+  const uint64_t wide = (uint64_t)nh * 192, narrow = (uint64_t)nh * 64;
+  int rc = make_tmap_bf16_2d(&m.qkv, qkv, (uint64_t)T, wide, wide, BW_TILE);
+  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.qkv_cols, qkv, (uint64_t)T, wide, wide, BW_COLS);
+  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.dout, dout, (uint64_t)T, narrow, narrow, BW_TILE);
+  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.dout_cols, dout, (uint64_t)T, narrow, narrow, BW_COLS);
+  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.dqkv, dqkv, (uint64_t)T, wide, wide, 32);
   if (rc != PE_OK) return rc;
   rc = set_max_dynamic_smem(reinterpret_cast<const void*>(attn_bwd_kernel), BW_SMEM, true);
   if (rc != PE_OK) return rc;
   BwArgs a;
   a.row_range = reinterpret_cast<const int2*>(ws + w.row_range);
   a.tile_range = reinterpret_cast<const int2*>(ws + w.tile_range);
-  a.lse2 = reinterpret_cast<const float*>(ws + w.lse2);
-  a.delta = reinterpret_cast<const float*>(ws + w.delta);
-  a.dqkv = static_cast<__nv_bfloat16*>(dqkv);
+  a.neg_lse2 = reinterpret_cast<const float*>(ws + w.lse2);
+  a.neg_delta = reinterpret_cast<const float*>(ws + w.delta);
   a.pos = position_ids;
   a.table = static_cast<const __nv_bfloat16*>(table);
   a.max_positions = max_positions;
@@ -659,10 +754,10 @@ extern "C" int pe_attn_varlen_backward(const void* dout, const void* qkv, const 
   attn_bwd_prepare_kernel<<<dim3((unsigned)tiles, (unsigned)nh), 256, 0, st>>>(
       static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), lse, cu_seqlens, n_seqs,
       (int)T, nh, half_window, const_cast<int2*>(a.row_range), const_cast<int2*>(a.tile_range),
-      const_cast<float*>(a.lse2), const_cast<float*>(a.delta), status);
+      const_cast<float*>(a.neg_lse2), const_cast<float*>(a.neg_delta), status);
   PE_LAUNCH_CHECK("attn_bwd_prepare_kernel");
   const int grid = (int)std::min<int64_t>(2 * int64_t(a.n_items), sm_count());
-  attn_bwd_kernel<<<grid, BW_THREADS, BW_SMEM, st>>>(tm_qkv, tm_dout, a);
+  attn_bwd_kernel<<<grid, BW_THREADS, BW_SMEM, st>>>(m, a);
   PE_LAUNCH_CHECK("attn_bwd_kernel");
   return PE_OK;
 }

@@ -77,6 +77,12 @@ def test_many_tiles_per_block(pe, cuda_device, hw):
     _check(lengths, 12, hw, cuda_device, seed=16)
 
 
+@pytest.mark.parametrize("hw", [None, 1500])
+def test_deep_column_walks(pe, cuda_device, hw):
+    """Blocks that walk hundreds of column tiles per item, several items each, row tiles of two sequences."""
+    _check([6000, 2100, 1], 4, hw, cuda_device, seed=17)
+
+
 @pytest.mark.parametrize("scale", [0.01, 4.0, 16.0])
 def test_flat_and_peaked_scores(pe, cuda_device, scale):
     _check([300, 40], 2, None, cuda_device, seed=5, scale=scale)
