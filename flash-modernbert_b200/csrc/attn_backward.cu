@@ -41,58 +41,55 @@ namespace pe {
 // 64-column buffers it needs beside the accumulators.
 constexpr int BW_GROUPS = 3;
 constexpr int BW_COMPUTE_WARPS = 4 * BW_GROUPS;
-// Beside them a producer warp and two warps that issue MMAs: one thread that waits, issues and commits
-// for all four products of a tile took longer over it than the tensor core.
 constexpr int BW_PRODUCER = BW_COMPUTE_WARPS;
-constexpr int BW_SCORES = BW_COMPUTE_WARPS + 1;      // S and dP
-constexpr int BW_ACCUMULATE = BW_COMPUTE_WARPS + 2;  // dV and dK, or dQ
-constexpr int BW_THREADS = 32 * (BW_COMPUTE_WARPS + 3);
+constexpr int BW_MMA = BW_COMPUTE_WARPS + 1;
+constexpr int BW_THREADS = 32 * (BW_COMPUTE_WARPS + 2);
 constexpr int BW_TILE = 128;                        // rows of a row tile
 constexpr int BW_COLS = 64;                         // columns of a column tile
 constexpr int BW_A_BYTES = BW_TILE * 64 * 2;        // one operand of a row tile
 constexpr int BW_B_BYTES = BW_COLS * 64 * 2;        // one operand of a column tile
-constexpr int BW_STAGES = 6;                        // column tiles in flight: (Q, dO) or (K, V)
+// The g-th column tile of a CTA belongs to group g % 3 and uses slot g % 6 of everything: the operand
+// ring in shared memory ((Q, dO) or (K, V), lse and delta), tensor memory and the barriers, whose
+// phases therefore all count g / 6.
+constexpr int BW_SLOTS = 2 * BW_GROUPS;
 constexpr int BW_STATS_BYTES = 2 * BW_COLS * 4;     // lse and delta of a column tile
-constexpr int BW_OUT_BYTES = 32 * 128;              // a warp's 32 rows of one gradient on their way out
+constexpr int BW_OUT_BYTES = 32 * 128;              // a compute warp's 32 rows of one gradient on their way out
 constexpr uint32_t BW_TMEM_COLS = 512;
-// Tensor memory: group w has two buffers of 64 columns at 128 w.  For its i-th tile the scores go to
-// buffer i % 2 and dP to the other.  The scores are replaced in place by P (32 columns of bf16 pairs)
-// and dS (32 more).  Once dP has been read its buffer takes the group's next scores; once P and dS have
-// been multiplied theirs takes the next dP.
+// Tensor memory: slots w and w + 3 are group w's two buffers of 64 columns, at 128 w and 64 further on.
+// The scores of a tile go to its own slot's buffer, dP to the group's other one.  The scores are
+// replaced in place by P (32 columns of bf16 pairs) and dS (32 more).  Once dP has been read its
+// buffer takes the group's next scores; once P and dS have been multiplied theirs takes the next dP.
 constexpr uint32_t BW_ACC1_COL = 384;  // dK or dQ
 constexpr uint32_t BW_ACC2_COL = 448;  // dV
 
-// Barriers of one pass; each pass has its own set.  [w]: one per group, whose phases the group's own
-// tiles (epilogues, for ACC_FULL) count, so that nobody who waits can be two phases behind.
+// Barriers of one pass; each pass has its own set.  [c]: one per slot.
 enum {
-  WB_FULL = 0,                           // [stage]
-  WB_EMPTY = WB_FULL + BW_STAGES,        // [stage]
-  WB_A_FULL = WB_EMPTY + BW_STAGES,      // [2]
-  WB_A_EMPTY = WB_A_FULL + 2,            // [2]
-  WB_S_FULL = WB_A_EMPTY + 2,            // [w]
-  WB_DP_FULL = WB_S_FULL + BW_GROUPS,    // [w]
-  WB_DK_DONE = WB_DP_FULL + BW_GROUPS,   // [w] a tile's dK (or dQ) has retired, and its dV before it
-  WB_ACC_FULL = WB_DK_DONE + BW_GROUPS,  // [w] the products of the item whose epilogue is w's have retired
+  WB_FULL = 0,                          // [c]
+  WB_EMPTY = WB_FULL + BW_SLOTS,        // [c]
+  WB_S_FULL = WB_EMPTY + BW_SLOTS,      // [c]
+  WB_DP_FULL = WB_S_FULL + BW_SLOTS,    // [c]
+  WB_DK_DONE = WB_DP_FULL + BW_SLOTS,   // [c] the tile's dK (or dQ) has retired, and all issued before it
+  WB_A_FULL = WB_DK_DONE + BW_SLOTS,    // [2]
+  WB_A_EMPTY = WB_A_FULL + 2,           // [2]
   // from here on: one arrival per warp of a group
-  // [2 w + parity of the group's tile] P written (key pass).  Two, because a group may reach its next
-  // tile's P before this tile's dV has been issued (but not the one after: that takes this tile's dK).
-  WB_P_FULL = WB_ACC_FULL + BW_GROUPS,
-  WB_DP_READ = WB_P_FULL + 2 * BW_GROUPS,  // [w]
-  WB_DS_FULL = WB_DP_READ + BW_GROUPS,   // [w]
-  WB_ACC_EMPTY = WB_DS_FULL + BW_GROUPS, // the item's accumulators have been read
-  WB_OUT_FREE = WB_ACC_EMPTY + 1,        // the item's gradients have left shared memory
-  WB_COUNT = WB_OUT_FREE + 1
+  WB_P_FULL = WB_A_EMPTY + 2,           // [c] P written (key pass)
+  WB_DP_READ = WB_P_FULL + BW_SLOTS,    // [c]
+  WB_DS_FULL = WB_DP_READ + BW_SLOTS,   // [c]
+  WB_ACC_EMPTY = WB_DS_FULL + BW_SLOTS, // the item's accumulators have been read
+  WB_COUNT = WB_ACC_EMPTY + 1
 };
-constexpr int BW_OUT_OFFSET = 4 * BW_A_BYTES + BW_STAGES * 2 * BW_B_BYTES;
-constexpr int BW_STATS_OFFSET = BW_OUT_OFFSET + 8 * BW_OUT_BYTES;
-constexpr int BW_BAR_OFFSET = BW_STATS_OFFSET + BW_STAGES * BW_STATS_BYTES;
+constexpr int BW_OUT_OFFSET = 4 * BW_A_BYTES + BW_SLOTS * 2 * BW_B_BYTES;
+constexpr int BW_STATS_OFFSET = BW_OUT_OFFSET + BW_COMPUTE_WARPS * BW_OUT_BYTES;
+constexpr int BW_BAR_OFFSET = BW_STATS_OFFSET + BW_SLOTS * BW_STATS_BYTES;
 constexpr int BW_SMEM = BW_BAR_OFFSET + 2 * WB_COUNT * 8 + 16;
+static_assert(BW_SMEM <= 227 * 1024, "shared memory of one CTA");
 
 struct BwArgs {
   const int2* row_range;    // [T]: columns [x, y) that row t attends
   const int2* tile_range;   // [tiles]: their union over a tile of 128 rows
   const float* neg_lse2;    // [nh, T]: -lse * log2(e)
   const float* neg_delta;   // [nh, T]
+  __nv_bfloat16* dqkv;      // [T, 3 nh 64]
   const int64_t* pos;       // [T] or NULL: rotation of q and k undone on dq and dk
   const __nv_bfloat16* table;
   int max_positions;
@@ -272,28 +269,41 @@ __device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, co
     }
   }
 }
-// Puts a row's 64 bf16 values (zeros if it is empty) into the warp's 128-byte-swizzled staging block.
-__device__ __forceinline__ void bw_stage_row(uint32_t block, int lane, const uint32_t (&v)[32], bool empty) {
+// Stores a warp's 32 rows of 64 bf16 values, a row per thread (zeros if it is empty): turned in the warp's
+// own block of shared memory, so that an instruction writes four whole 128-byte rows.  `dst` is the
+// first row's, `rows` how many of them exist.
+__device__ __forceinline__ void bw_store_rows(__nv_bfloat16* dst, int64_t ld, int rows, uint32_t block, int lane,
+                                              const uint32_t (&v)[32], bool empty) {
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(block + lane * 128 + ((i ^ (lane & 7)) << 4)),
                  "r"(empty ? 0u : v[4 * i]), "r"(empty ? 0u : v[4 * i + 1]), "r"(empty ? 0u : v[4 * i + 2]),
                  "r"(empty ? 0u : v[4 * i + 3])
                  : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    uint4 u;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                 : "r"(block + r * 128 + (((lane & 7) ^ (r & 7)) << 4))
+                 : "memory");
+    if (r < rows) *reinterpret_cast<uint4*>(dst + r * ld + (lane & 7) * 8) = u;
+  }
+  __syncwarp();
 }
-
-struct BwMaps {  // rows x 64 columns: row tiles (128), column tiles (64), a warp's rows of the result (32)
-  CUtensorMap qkv, qkv_cols, dout, dout_cols, dqkv;
-};
 
 // KEYS: the key pass (rows are keys, columns are queries), else the query pass.  `first` is this
 // CTA's first item.  Returns false if a bounded wait gave up.
 template <bool KEYS>
-__device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int first, uint32_t base,
-                                        uint32_t bar_base, uint32_t tmem_base) {
+__device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtensorMap& tm_qkv_cols,
+                                        const CUtensorMap& tm_dout, const CUtensorMap& tm_dout_cols,
+                                        const BwArgs& a, int first, uint32_t base, uint32_t bar_base,
+                                        uint32_t tmem_base) {
   auto bar = [&](int i) { return bar_base + 8u * i; };
   const uint32_t sA = base;                  // A[buffer]: (K, V) or (Q, dO)
-  const uint32_t sB = base + 4 * BW_A_BYTES; // B[stage]: (Q, dO) or (K, V)
+  const uint32_t sB = base + 4 * BW_A_BYTES; // B[slot]: (Q, dO) or (K, V)
   const uint32_t sStats = base + BW_STATS_OFFSET;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int H = a.nh * 64;
@@ -304,144 +314,157 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
 
   if (warp == BW_PRODUCER) {
     // ---------------------------------------------------------------- producer
-    uint32_t st = 0, phase = 0, loads = 0, ord = 0;
+    uint32_t c = 0, lap = 0, loads = 0, ord = 0;
     for (; it.valid(a) && ok; it.next(a), ++ord) {
       const uint32_t ab = ord & 1;
-      const int c = it.head * 64, row0 = it.tile * BW_TILE;
+      const int col = it.head * 64, row0 = it.tile * BW_TILE;
       if (!mbar_wait(bar(WB_A_EMPTY + ab), ((ord >> 1) & 1) ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
       if (lane == 0) {
         const uint32_t dst = sA + ab * 2 * BW_A_BYTES;
         mbar_expect_tx(bar(WB_A_FULL + ab), 2 * BW_A_BYTES);
-        tma_load_2d(dst, &m.qkv, bar(WB_A_FULL + ab), (KEYS ? H : 0) + c, row0);
-        if (KEYS) tma_load_2d(dst + BW_A_BYTES, &m.qkv, bar(WB_A_FULL + ab), 2 * H + c, row0);
-        else tma_load_2d(dst + BW_A_BYTES, &m.dout, bar(WB_A_FULL + ab), c, row0);
+        tma_load_2d(dst, &tm_qkv, bar(WB_A_FULL + ab), (KEYS ? H : 0) + col, row0);
+        if (KEYS) tma_load_2d(dst + BW_A_BYTES, &tm_qkv, bar(WB_A_FULL + ab), 2 * H + col, row0);
+        else tma_load_2d(dst + BW_A_BYTES, &tm_dout, bar(WB_A_FULL + ab), col, row0);
       }
       __syncwarp();
       const float* lse_head = a.neg_lse2 + int64_t(it.head) * a.T;
       const float* delta_head = a.neg_delta + int64_t(it.head) * a.T;
       for (int j = 0; j < it.n; ++j) {
-        if (!mbar_wait(bar(WB_EMPTY + st), phase ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
+        if (!mbar_wait(bar(WB_EMPTY + c), (lap & 1) ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
         const int col0 = it.col0(j);
         if (KEYS) {
 #pragma unroll
           for (int i = 0; i < BW_COLS / 32; ++i) {
             const int q = min(max(col0 + i * 32 + lane, 0), a.T - 1);
-            const uint32_t dst = sStats + st * BW_STATS_BYTES + (i * 32 + lane) * 4;
+            const uint32_t dst = sStats + c * BW_STATS_BYTES + (i * 32 + lane) * 4;
             cp_async4(dst, lse_head + q);
             cp_async4(dst + BW_COLS * 4, delta_head + q);
           }
-          cp_async_arrive(bar(WB_FULL + st));
+          cp_async_arrive(bar(WB_FULL + c));
         }
         if (lane == 0) {
-          const uint32_t dst = sB + st * 2 * BW_B_BYTES;
-          mbar_expect_tx(bar(WB_FULL + st), 2 * BW_B_BYTES);
-          tma_load_2d(dst, &m.qkv_cols, bar(WB_FULL + st), (KEYS ? 0 : H) + c, col0);
-          if (KEYS) tma_load_2d(dst + BW_B_BYTES, &m.dout_cols, bar(WB_FULL + st), c, col0);
-          else tma_load_2d(dst + BW_B_BYTES, &m.qkv_cols, bar(WB_FULL + st), 2 * H + c, col0);
+          const uint32_t dst = sB + c * 2 * BW_B_BYTES;
+          mbar_expect_tx(bar(WB_FULL + c), 2 * BW_B_BYTES);
+          tma_load_2d(dst, &tm_qkv_cols, bar(WB_FULL + c), (KEYS ? 0 : H) + col, col0);
+          if (KEYS) tma_load_2d(dst + BW_B_BYTES, &tm_dout_cols, bar(WB_FULL + c), col, col0);
+          else tma_load_2d(dst + BW_B_BYTES, &tm_qkv_cols, bar(WB_FULL + c), 2 * H + col, col0);
         }
         __syncwarp();
         ++loads;
-        if (++st == BW_STAGES) {
-          st = 0;
-          phase ^= 1u;
+        if (++c == BW_SLOTS) {
+          c = 0;
+          ++lap;
         }
       }
     }
     if (!ok) {  // gave up: this CTA's copies must have landed before it can leave
-      for (uint32_t u = loads > BW_STAGES ? loads - BW_STAGES : 0; u < loads; ++u)
-        mbar_wait(bar(WB_FULL + u % BW_STAGES), (u / BW_STAGES) & 1, status, ST_ATTN_TIMEOUT);
+      for (uint32_t u = loads > BW_SLOTS ? loads - BW_SLOTS : 0; u < loads; ++u)
+        mbar_wait(bar(WB_FULL + u % BW_SLOTS), (u / BW_SLOTS) & 1, status, ST_ATTN_TIMEOUT);
       for (uint32_t u = ord > 1 ? ord - 2 : 0; u <= ord; ++u)  // (one that was never issued runs into its limit)
         mbar_wait(bar(WB_A_FULL + (u & 1)), (u >> 1) & 1, status, ST_ATTN_TIMEOUT);
     }
-  } else if (warp == BW_SCORES) {
-    // ---------------------------------------------------------------- S and dP
+  } else if (warp == BW_MMA) {
+    // ---------------------------------------------------------------- MMA issuer
+    // The scores run three tiles ahead of the accumulation and dP two, so that by the time something
+    // is waited for it has usually happened: this one thread feeds the tensor core with four
+    // products per tile and its own latency counts.
     if (elect_one()) {
-      constexpr uint32_t idesc = umma_idesc_bf16(BW_TILE, BW_COLS, 0);
+      constexpr uint32_t idesc_s = umma_idesc_bf16(BW_TILE, BW_COLS, 0);
+      constexpr uint32_t idesc_acc = umma_idesc_bf16(BW_TILE, 64, 1);  // B is MN-major: its rows are the contraction
       auto wait = [&](int b, uint32_t parity) {
-        if (!mbar_wait(bar(b), parity, status, ST_ATTN_MMA_TIMEOUT)) ok = false;
+        if (ok && !mbar_wait(bar(b), parity, status, ST_ATTN_MMA_TIMEOUT)) ok = false;
         return ok;
       };
-      auto product = [&](uint32_t d_col, uint64_t ad, uint64_t bd) {
+      auto buffer = [&](uint32_t c) { return tmem_base + (c >= BW_GROUPS ? (c - BW_GROUPS) * 128 + 64 : c * 128); };
+      const uint64_t a_desc = umma_smem_desc_sw128(sA, 1024), b_desc = umma_smem_desc_sw128(sB, 1024);
+      auto scores = [&](uint32_t d, uint64_t ad, uint64_t bd) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_ss(tmem_base + d_col, ad + 2u * kk, bd + 2u * kk, idesc, kk != 0 ? 1u : 0u);
-      };
-      // group, its tile's parity, stage and its phase of the tile about to be issued
-      uint32_t w = 0, i = 0, st = 0, phase = 0, ord = 0;
-      for (; it.valid(a) && ok; it.next(a), ++ord) {
-        const uint64_t a1 = umma_smem_desc_sw128(sA + (ord & 1) * 2 * BW_A_BYTES, 1024);
-        const uint64_t a2 = umma_smem_desc_sw128(sA + ((ord & 1) * 2 + 1) * BW_A_BYTES, 1024);
-        if (!wait(WB_A_FULL + (ord & 1), (ord >> 1) & 1)) break;
-        for (int j = 0; j < it.n; ++j) {
-          const uint64_t b1 = umma_smem_desc_sw128(sB + st * 2 * BW_B_BYTES, 1024);
-          const uint32_t s_col = w * 128 + (i & 1) * 64;
-          if (!wait(WB_FULL + st, phase)) break;
-          // the group's last dP has been read: its buffer takes these scores
-          if (i > 0 && !wait(WB_DP_READ + w, (i & 1) ^ 1u)) break;
-          tc_fence_after();
-          product(s_col, a1, b1);
-          umma_commit(bar(WB_S_FULL + w));
-          // the group's last P and dS have been multiplied: their buffer takes this dP
-          if (i > 0 && !wait(WB_DK_DONE + w, (i & 1) ^ 1u)) break;
-          tc_fence_after();
-          product(s_col ^ 64u, a2, b1 + (BW_B_BYTES >> 4));
-          umma_commit(bar(WB_DP_FULL + w));
-          if (++w == BW_GROUPS) {
-            w = 0;
-            ++i;
-          }
-          if (++st == BW_STAGES) {
-            st = 0;
-            phase ^= 1u;
-          }
-        }
-        if (ok) umma_commit(bar(WB_A_EMPTY + (ord & 1)));
-      }
-    }
-    __syncwarp();
-    ok = __all_sync(0xffffffffu, ok);
-  } else if (warp == BW_ACCUMULATE) {
-    // ---------------------------------------------------------------- dV and dK, or dQ
-    if (elect_one()) {
-      constexpr uint32_t idesc = umma_idesc_bf16(BW_TILE, 64, 1);  // B is MN-major: its rows are the contraction
-      auto wait = [&](int b, uint32_t parity) {
-        if (!mbar_wait(bar(b), parity, status, ST_ATTN_MMA_TIMEOUT)) ok = false;
-        return ok;
+        for (int kk = 0; kk < 4; ++kk) umma_ss(d, ad + 2u * kk, bd + 2u * kk, idesc_s, kk != 0 ? 1u : 0u);
       };
       // acc += X B, X (bf16 pairs of 64 columns) in tensor memory
-      auto accumulate = [&](uint32_t acc_col, uint32_t x_col, uint64_t bd, bool first_tile) {
+      auto accumulate = [&](uint32_t acc_col, uint32_t x, uint64_t bd, bool first_tile) {
 #pragma unroll
         for (int kk = 0; kk < BW_COLS / 16; ++kk)
-          g_umma_ts(tmem_base + acc_col, tmem_base + x_col + kk * 8, bd + uint32_t(kk * 2048 >> 4), idesc,
+          g_umma_ts(tmem_base + acc_col, x + kk * 8, bd + uint32_t(kk * 2048 >> 4), idesc_acc,
                     (!first_tile || kk != 0) ? 1u : 0u);
       };
-      uint32_t w = 0, i = 0, st = 0, phase = 0, ord = 0;
-      for (; it.valid(a) && ok; it.next(a), ++ord) {
-        // the previous item's accumulators must have been read before they are overwritten
-        if (ord > 0 && !wait(WB_ACC_EMPTY, (ord & 1) ^ 1u)) break;
-        for (int j = 0; j < it.n; ++j) {
-          const uint64_t b1 = umma_smem_desc_sw128(sB + st * 2 * BW_B_BYTES, 1024);
-          const uint32_t s_col = w * 128 + (i & 1) * 64;
-          if (!wait(WB_FULL + st, phase)) break;
-          if (KEYS) {
-            if (!wait(WB_P_FULL + 2 * w + (i & 1), (i >> 1) & 1)) break;
-            tc_fence_after();
-            accumulate(BW_ACC2_COL, s_col, b1 + (BW_B_BYTES >> 4), j == 0);  // dV += P^T dO
-          }
-          if (!wait(WB_DS_FULL + w, i & 1)) break;
+      // A tile on its way from scores to accumulation: A buffer (1), first (2) and last (4) of its
+      // item, present (8)
+      int j = 0;
+      uint32_t ord = 0, a_loads = 0;
+      auto next_tile = [&]() {
+        if (!it.valid(a)) return 0u;
+        const uint32_t f = 8u | (ord & 1) | (j == 0 ? 2u : 0u) | (j + 1 == it.n ? 4u : 0u);
+        if (++j == it.n) {
+          j = 0;
+          ++ord;
+          it.next(a);
+        }
+        return f;
+      };
+      auto issue_s = [&](uint32_t f, uint32_t c, uint32_t lap) {  // of the tile in slot c
+        if (f & 2u) {
+          if (!wait(WB_A_FULL + (f & 1), (a_loads >> 1) & 1)) return;
+          ++a_loads;
+        }
+        if (!wait(WB_FULL + c, lap & 1)) return;
+        tc_fence_after();
+        scores(buffer(c), a_desc + (f & 1) * (2 * BW_A_BYTES >> 4), b_desc + c * (2 * BW_B_BYTES >> 4));
+        umma_commit(bar(WB_S_FULL + c));
+      };
+      auto issue_dp = [&](uint32_t f, uint32_t c) {  // its operands arrived with those of its scores
+        scores(buffer(c) ^ 64u, a_desc + ((f & 1) * 2 + 1) * (BW_A_BYTES >> 4),
+               b_desc + (c * 2 + 1) * (BW_B_BYTES >> 4));
+        umma_commit(bar(WB_DP_FULL + c));
+        if (f & 4u) umma_commit(bar(WB_A_EMPTY + (f & 1)));
+      };
+      uint32_t f0 = next_tile(), f1 = next_tile(), f2 = next_tile();  // tiles g, g + 1, g + 2
+      if (f0) {
+        issue_s(f0, 0, 0);
+        if (ok) issue_dp(f0, 0);
+      }
+      if (f1 && ok) {
+        issue_s(f1, 1, 0);
+        if (ok) issue_dp(f1, 1);
+      }
+      if (f2 && ok) issue_s(f2, 2, 0);
+      uint32_t c = 0, lap = 0, items = 0;  // slot and lap of tile g, items whose accumulation has begun
+      while (ok && f0) {
+        const uint64_t b1 = b_desc + c * (2 * BW_B_BYTES >> 4);
+        const bool fresh = (f0 & 2u) != 0;
+        if (fresh) {  // the previous item's accumulators must have been read before they are overwritten
+          if (items > 0 && !wait(WB_ACC_EMPTY, (items - 1) & 1)) break;
+          ++items;
+        }
+        if (KEYS) {
+          if (!wait(WB_P_FULL + c, lap & 1)) break;
           tc_fence_after();
-          accumulate(BW_ACC1_COL, s_col + 32, b1, j == 0);  // dK += dS^T Q, dQ += dS K
-          umma_commit(bar(WB_DK_DONE + w));
-          umma_commit(bar(WB_EMPTY + st));
-          if (j + 1 == it.n) umma_commit(bar(WB_ACC_FULL + w));
-          if (++w == BW_GROUPS) {
-            w = 0;
-            ++i;
-          }
-          if (++st == BW_STAGES) {
-            st = 0;
-            phase ^= 1u;
-          }
+          accumulate(BW_ACC2_COL, buffer(c), b1 + (BW_B_BYTES >> 4), fresh);  // dV += P^T dO
+        }
+        const uint32_t f3 = next_tile();
+        if (f3) {  // dP of tile g has been read: its buffer takes the scores of tile g + 3
+          const uint32_t c3 = c >= BW_GROUPS ? c - BW_GROUPS : c + BW_GROUPS;
+          if (!wait(WB_DP_READ + c, lap & 1)) break;
+          issue_s(f3, c3, lap + (c >= BW_GROUPS ? 1 : 0));
+          if (!ok) break;
+        }
+        if (f2) {  // P and dS of tile g - 1 have been multiplied: their buffer takes dP of tile g + 2
+          const uint32_t cm = c == 0 ? BW_SLOTS - 1 : c - 1;
+          if ((c | lap) != 0 && !wait(WB_DK_DONE + cm, (lap - (c == 0 ? 1 : 0)) & 1)) break;
+          tc_fence_after();
+          issue_dp(f2, c + 2 >= BW_SLOTS ? c + 2 - BW_SLOTS : c + 2);
+        }
+        if (!wait(WB_DS_FULL + c, lap & 1)) break;
+        tc_fence_after();
+        accumulate(BW_ACC1_COL, buffer(c) + 32, b1, fresh);  // dK += dS^T Q, dQ += dS K
+        umma_commit(bar(WB_DK_DONE + c));
+        umma_commit(bar(WB_EMPTY + c));
+        f0 = f1;
+        f1 = f2;
+        f2 = f3;
+        if (++c == BW_SLOTS) {
+          c = 0;
+          ++lap;
         }
       }
     }
@@ -452,7 +475,7 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
     const int w = warp >> 2;                         // group
     const int row = (warp & 3) * 32 + lane;          // row of the tile = tensor-memory lane
     const uint32_t lane_addr = tmem_base + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t out_block = base + BW_OUT_OFFSET + (warp & 3) * 2 * BW_OUT_BYTES;
+    const uint32_t out_block = base + BW_OUT_OFFSET + warp * BW_OUT_BYTES;
     const float scale_log2 = 0.125f * 1.4426950408889634f;  // 1/sqrt(64) * log2(e)
     const float2 scale2 = make_float2(scale_log2, scale_log2);
     // After a bounded wait has given up the loops still run to their end, without waiting, so that
@@ -465,11 +488,9 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(b));
     };
-    int j = w;                                 // this group's next tile, counted from the item's first
-    uint32_t i = 0, epilogues = 0, ord = 0;    // tiles and epilogues of this group, items so far
-    uint32_t st = w;                           // stage of tile j and how often its ring has gone round
-    uint32_t round = 0;
-    for (; it.valid(a); it.next(a), ++ord) {
+    int j = w;       // this group's next tile, counted from the item's first
+    uint32_t i = 0;  // tiles of this group so far
+    for (; it.valid(a); it.next(a)) {
       if (j < it.n) {
         // what this thread's row brings along
         const int t = it.tile * BW_TILE + row;
@@ -484,15 +505,16 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
           }
         }
         for (; j < it.n; j += BW_GROUPS, ++i) {
+          const uint32_t c = w + (i & 1) * BW_GROUPS, lap = (i >> 1) & 1;
           const uint32_t s_addr = lane_addr + w * 128 + (i & 1) * 64;
           const uint32_t dp_addr = s_addr ^ 64u;
-          const uint32_t stats = sStats + st * BW_STATS_BYTES;
+          const uint32_t stats = sStats + c * BW_STATS_BYTES;
           // valid columns of this row within the tile: [c_lo, c_hi)
           const int x0 = it.col0(j);
           const int c_lo = max(range.x, it.lo + j * BW_COLS) - x0, c_hi = range.y - x0;
           const bool full = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= BW_COLS);
-          wait(WB_S_FULL + w, i & 1);
-          if (KEYS) wait(WB_FULL + st, round & 1);  // complete by now: makes lse and delta visible
+          wait(WB_S_FULL + c, lap);
+          if (KEYS) wait(WB_FULL + c, lap);  // complete by now: makes lse and delta visible
           tc_fence_after();
           uint32_t p[64];
           g_tmem_ld32(s_addr, p);
@@ -531,9 +553,9 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
               g_tmem_st16(s_addr + h * 16, pk);
             }
             g_tmem_st_wait();
-            arrive(WB_P_FULL + 2 * w + (i & 1));
+            arrive(WB_P_FULL + c);
           }
-          wait(WB_DP_FULL + w, i & 1);
+          wait(WB_DP_FULL + c, lap);
           tc_fence_after();
           uint32_t dp[2][16];
           g_tmem_ld16(dp_addr, dp[0]);
@@ -541,7 +563,7 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
           for (int h = 0; h < 4; ++h) {
             tmem_ld_wait();
             if (h < 3) g_tmem_ld16(dp_addr + (h + 1) * 16, dp[(h + 1) & 1]);  // in flight during this quarter
-            else arrive(WB_DP_READ + w);
+            else arrive(WB_DP_READ + c);
             const uint32_t* d = dp[h & 1];
             uint32_t pk[8];
 #pragma unroll
@@ -562,16 +584,11 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
             g_tmem_st8(s_addr + 32 + h * 8, pk);  // dS in place of the second half
           }
           g_tmem_st_wait();
-          arrive(WB_DS_FULL + w);
-          st += BW_GROUPS;
-          if (st >= BW_STAGES) {
-            st -= BW_STAGES;
-            ++round;
-          }
+          arrive(WB_DS_FULL + c);
           if (j + 1 == it.n) {
             // The group of an item's last tile stores its gradients while the others go on; the row's 64
             // (or twice 64) values are in registers before the accumulators are handed back.  Rows
-            // that attend nothing are exact zeros; rows beyond T are clipped by the store.
+            // that attend nothing are exact zeros.
             const uint4* trow = nullptr;
             if (a.pos != nullptr && t < a.T) {
               int64_t ps = a.pos[t];
@@ -581,45 +598,32 @@ __device__ __forceinline__ bool bw_pass(const BwMaps& m, const BwArgs& a, int fi
               }
               trow = reinterpret_cast<const uint4*>(a.table + ps * 64);
             }
-            wait(WB_ACC_FULL + w, epilogues & 1);
-            ++epilogues;
+            wait(WB_DK_DONE + c, lap);
             tc_fence_after();
             uint32_t v1[32], v2[32];
             bw_finish_row(lane_addr + BW_ACC1_COL, 0.125f, trow, v1);
             if (KEYS) bw_finish_row(lane_addr + BW_ACC2_COL, 1.0f, nullptr, v2);
-            // The staging blocks are shared by the groups.  (Waited for before the accumulators are handed
-            // back, so that the group of the next item finds at most this item's phase pending.)
-            if (ord > 0) wait(WB_OUT_FREE, (ord & 1) ^ 1u);
             arrive(WB_ACC_EMPTY);
             const bool empty = range.x >= range.y;
-            bw_stage_row(out_block, lane, v1, empty);
-            if (KEYS) bw_stage_row(out_block + BW_OUT_BYTES, lane, v2, empty);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              const int row0 = it.tile * BW_TILE + (warp & 3) * 32;
-              if (ok && row0 < a.T) {
-                tma_store_2d(&m.dqkv, out_block, (KEYS ? H : 0) + it.head * 64, row0);
-                if (KEYS) tma_store_2d(&m.dqkv, out_block + BW_OUT_BYTES, 2 * H + it.head * 64, row0);
-                tma_store_commit();
-                tma_store_wait_read<0>();
-              }
-              mbar_arrive(bar(WB_OUT_FREE));
-            }
-            __syncwarp();
+            const int row0 = it.tile * BW_TILE + (warp & 3) * 32;
+            const int rows = ok ? a.T - row0 : 0;
+            const int64_t ld = 3 * int64_t(H);
+            __nv_bfloat16* dst = a.dqkv + row0 * ld + (KEYS ? H : 0) + it.head * 64;
+            bw_store_rows(dst, ld, rows, out_block, lane, v1, empty);
+            if (KEYS) bw_store_rows(dst + H, ld, rows, out_block, lane, v2, empty);
           }
         }
       }
       j -= it.n;
     }
-    if (lane == 0) tma_store_wait_all<0>();  // staging memory must outlive the stores that read it
-    __syncwarp();
   }
   return ok;
 }
 
 __global__ void __launch_bounds__(BW_THREADS, 1)
-attn_bwd_kernel(const __grid_constant__ BwMaps m, const BwArgs a) {
+attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_qkv_cols,
+                const __grid_constant__ CUtensorMap tm_dout, const __grid_constant__ CUtensorMap tm_dout_cols,
+                const BwArgs a) {
   extern __shared__ __align__(1024) uint8_t bw_smem[];
   const uint32_t base = smem_u32(bw_smem);
   if (base & 1023u) {  // the swizzled tiles need it; nothing has been allocated yet
@@ -635,19 +639,18 @@ attn_bwd_kernel(const __grid_constant__ BwMaps m, const BwArgs a) {
       for (int i = 0; i < WB_COUNT; ++i) {
         uint32_t count = 1;
         // stages of the key pass: the TMA issue and 32 lanes' copies of lse and delta
-        if (pass == 0 && i >= WB_FULL && i < WB_FULL + BW_STAGES) count = 33;
+        if (pass == 0 && i >= WB_FULL && i < WB_FULL + BW_SLOTS) count = 33;
         if (i >= WB_P_FULL) count = 4;
         mbar_init(bb + 8u * i, count);
       }
     }
     mbar_fence_init();
-    tma_prefetch_desc(&m.qkv);
-    tma_prefetch_desc(&m.qkv_cols);
-    tma_prefetch_desc(&m.dout);
-    tma_prefetch_desc(&m.dout_cols);
-    tma_prefetch_desc(&m.dqkv);
+    tma_prefetch_desc(&tm_qkv);
+    tma_prefetch_desc(&tm_qkv_cols);
+    tma_prefetch_desc(&tm_dout);
+    tma_prefetch_desc(&tm_dout_cols);
   }
-  if (warp == BW_ACCUMULATE) {
+  if (warp == BW_MMA) {
     tmem_alloc(tmem_slot, BW_TMEM_COLS);
     tmem_relinquish();
   }
@@ -659,18 +662,18 @@ attn_bwd_kernel(const __grid_constant__ BwMaps m, const BwArgs a) {
 
   // Items of both passes form one list, the key pass first; a CTA takes every gridDim-th of it, so
   // the passes need no launch boundary and a small batch runs both at the same time.
-  const bool ok = bw_pass<true>(m, a, blockIdx.x, base, bar_base, tmem_base);
+  const bool ok = bw_pass<true>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, blockIdx.x, base, bar_base, tmem_base);
   tc_fence_before();
   const int failed = __syncthreads_or(!ok);
   tc_fence_after();
   if (!failed) {
     int first = int(blockIdx.x) - a.n_items % int(gridDim.x);
     if (first < 0) first += gridDim.x;
-    bw_pass<false>(m, a, first, base, bar_base + WB_COUNT * 8, tmem_base);
+    bw_pass<false>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, first, base, bar_base + WB_COUNT * 8, tmem_base);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == BW_ACCUMULATE) {
+  if (warp == BW_MMA) {
     tc_fence_after();
     tmem_dealloc(tmem_base, BW_TMEM_COLS);
   }
@@ -729,13 +732,12 @@ extern "C" int pe_attn_varlen_backward(const void* dout, const void* qkv, const 
   if (T == 0) return PE_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  BwMaps m;
+  CUtensorMap tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols;
   const uint64_t wide = (uint64_t)nh * 192, narrow = (uint64_t)nh * 64;
-  int rc = make_tmap_bf16_2d(&m.qkv, qkv, (uint64_t)T, wide, wide, BW_TILE);
-  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.qkv_cols, qkv, (uint64_t)T, wide, wide, BW_COLS);
-  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.dout, dout, (uint64_t)T, narrow, narrow, BW_TILE);
-  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.dout_cols, dout, (uint64_t)T, narrow, narrow, BW_COLS);
-  if (rc == PE_OK) rc = make_tmap_bf16_2d(&m.dqkv, dqkv, (uint64_t)T, wide, wide, 32);
+  int rc = make_tmap_bf16_2d(&tm_qkv, qkv, (uint64_t)T, wide, wide, BW_TILE);
+  if (rc == PE_OK) rc = make_tmap_bf16_2d(&tm_qkv_cols, qkv, (uint64_t)T, wide, wide, BW_COLS);
+  if (rc == PE_OK) rc = make_tmap_bf16_2d(&tm_dout, dout, (uint64_t)T, narrow, narrow, BW_TILE);
+  if (rc == PE_OK) rc = make_tmap_bf16_2d(&tm_dout_cols, dout, (uint64_t)T, narrow, narrow, BW_COLS);
   if (rc != PE_OK) return rc;
   rc = set_max_dynamic_smem(reinterpret_cast<const void*>(attn_bwd_kernel), BW_SMEM, true);
   if (rc != PE_OK) return rc;
@@ -743,6 +745,7 @@ extern "C" int pe_attn_varlen_backward(const void* dout, const void* qkv, const 
   a.row_range = reinterpret_cast<const int2*>(ws + w.row_range);
   a.tile_range = reinterpret_cast<const int2*>(ws + w.tile_range);
   a.neg_lse2 = reinterpret_cast<const float*>(ws + w.lse2);
+  a.dqkv = static_cast<__nv_bfloat16*>(dqkv);
   a.neg_delta = reinterpret_cast<const float*>(ws + w.delta);
   a.pos = position_ids;
   a.table = static_cast<const __nv_bfloat16*>(table);
@@ -757,7 +760,7 @@ extern "C" int pe_attn_varlen_backward(const void* dout, const void* qkv, const 
       const_cast<float*>(a.neg_lse2), const_cast<float*>(a.neg_delta), status);
   PE_LAUNCH_CHECK("attn_bwd_prepare_kernel");
   const int grid = (int)std::min<int64_t>(2 * int64_t(a.n_items), sm_count());
-  attn_bwd_kernel<<<grid, BW_THREADS, BW_SMEM, st>>>(m, a);
+  attn_bwd_kernel<<<grid, BW_THREADS, BW_SMEM, st>>>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a);
   PE_LAUNCH_CHECK("attn_bwd_kernel");
   return PE_OK;
 }
