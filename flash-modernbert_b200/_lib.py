@@ -180,6 +180,13 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def device_stream_ptr(index: int) -> int:
+    """The current stream of device `index`, without the Python stream object in between."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def current_stream_ptr() -> int:
     import torch
 

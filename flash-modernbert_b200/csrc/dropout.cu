@@ -9,6 +9,7 @@
 // allows, and a drop probability in steps of 2^-16 is finer than anyone sets it.  Survivors
 // are scaled by what that rounded probability makes of them, so the expectation is exact.
 #include <algorithm>
+#include <type_traits>
 
 #include "pe_host.h"
 #include "pe_vec.cuh"
@@ -36,68 +37,82 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, PhiloxKeys k) {
   return make_uint4(c0, c1, c2, c3);
 }
 
-// Eight consecutive elements as fp32 and back, one rounding to nearest even.
+// Eight consecutive elements: as they lie in memory, and as fp32 (back with one rounding to nearest even).
 template <typename E>
-struct Octet;
-template <>
-struct Octet<__nv_bfloat16> {
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&f)[8]) {
-    unpack8(ld_stream(reinterpret_cast<const uint4*>(p)), f);
-  }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[8]) {
-    *reinterpret_cast<uint4*>(p) = pack8(f);
-  }
-  static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-  static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-};
-template <>
-struct Octet<__half> {
-  static __device__ __forceinline__ void load(const __half* p, float (&f)[8]) {
-    const uint4 v = ld_stream(reinterpret_cast<const uint4*>(p));
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
+struct Octet {
+  static constexpr int VECS = int(sizeof(E)) / 2;
+  uint4 u[VECS];
+  __device__ __forceinline__ void load(const E* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = __half22float2(h[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
+    for (int i = 0; i < VECS; ++i) u[i] = ld_stream(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void store(E* p) const {
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
+  }
+  __device__ __forceinline__ void unpack(float (&f)[8]) const {
+    if constexpr (std::is_same<E, float>::value) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = reinterpret_cast<const float*>(u)[i];
+    } else if constexpr (std::is_same<E, __half>::value) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(reinterpret_cast<const __half2*>(u)[i]);
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+      }
+    } else {
+      unpack8(u[0], f);
     }
   }
-  static __device__ __forceinline__ void store(__half* p, const float (&f)[8]) {
-    uint4 v;
-    __half2* h = reinterpret_cast<__half2*>(&v);
+  __device__ __forceinline__ void pack(const float (&f)[8]) {
+    if constexpr (std::is_same<E, float>::value) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = v;
-  }
-  static __device__ __forceinline__ float get(const __half* p) { return __half2float(*p); }
-  static __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-};
-template <>
-struct Octet<float> {
-  static __device__ __forceinline__ void load(const float* p, float (&f)[8]) {
+      for (int i = 0; i < 8; ++i) reinterpret_cast<float*>(u)[i] = f[i];
+    } else if constexpr (std::is_same<E, __half>::value) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 v = ld_stream(reinterpret_cast<const uint4*>(p) + i);
-      f[4 * i] = __uint_as_float(v.x);
-      f[4 * i + 1] = __uint_as_float(v.y);
-      f[4 * i + 2] = __uint_as_float(v.z);
-      f[4 * i + 3] = __uint_as_float(v.w);
+      for (int i = 0; i < 4; ++i) reinterpret_cast<__half2*>(u)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    } else {
+      u[0] = pack8(f);
     }
   }
-  static __device__ __forceinline__ void store(float* p, const float (&f)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  }
-  static __device__ __forceinline__ float get(const float* p) { return *p; }
-  static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 };
+__device__ __forceinline__ float element_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float element_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float element_f32(float v) { return v; }
+__device__ __forceinline__ void element_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void element_put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void element_put(float* p, float v) { *p = v; }
 
-// VECTOR: every pointer is 16-byte aligned, whole octets move in 16-byte pieces (the last, partial
-// one element by element).  Dropped elements are selected away, not multiplied by zero, so a
-// NaN or infinity among them leaves no trace.
+// y of eight elements, in place of x.  A 16-bit field is compared where it stands: the high half of a word
+// is at least t if the word is at least t 2^16, the low half after a shift.  Dropped elements are
+// selected away, not multiplied by zero, so a NaN or infinity among them leaves no trace.
+template <bool RESIDUAL>
+__device__ __forceinline__ void dropout_octet(float (&v)[8], const float (&r)[8], uint4 bits, uint32_t threshold_hi,
+                                              bool all, float scale) {
+  const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = __fmul2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(scale, scale));
+    v[2 * i] = !all && (word[i] << 16) >= threshold_hi ? u.x : 0.f;
+    v[2 * i + 1] = !all && word[i] >= threshold_hi ? u.y : 0.f;
+    if (RESIDUAL) {
+      v[2 * i] += r[2 * i];
+      v[2 * i + 1] += r[2 * i + 1];
+    }
+  }
+}
+
+// VECTOR: every pointer is 16-byte aligned, whole octets move in 16-byte pieces (the last, partial one
+// element by element).  threshold_hi: the drop threshold times 2^16; `all`: everything is dropped.
+// VECTOR: every pointer is 16-byte aligned, whole octets move in 16-byte pieces (the last, partial one
+// element by element).  threshold_hi: the drop threshold times 2^16; `all`: everything is dropped.
+// Eight blocks per SM, all 64 warps, hide the generator's latency; two octets per thread and step, or the next
+// octet's loads issued a step ahead, cost the registers that the warps need and were slower
+// (306,851 x 768 bf16: 193 us as it is, 196 - 212 us so).
 template <typename E, bool RESIDUAL, bool VECTOR>
-__global__ void __launch_bounds__(256)
-dropout_kernel(const E* x, const E* residual, E* y, int64_t n, uint32_t threshold, float scale,
+__global__ void __launch_bounds__(256, 8)
+dropout_kernel(const E* x, const E* residual, E* y, int64_t n, uint32_t threshold_hi, bool all, float scale,
                const int64_t* __restrict__ rng, int64_t* __restrict__ rng_used) {
   const uint64_t seed = uint64_t(__ldg(rng)), position = uint64_t(__ldg(rng + 1));
   if (rng_used != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
@@ -110,32 +125,32 @@ dropout_kernel(const E* x, const E* residual, E* y, int64_t n, uint32_t threshol
        o += int64_t(gridDim.x) * blockDim.x) {
     const int64_t at = o * 8;
     const int count = int(n - at < 8 ? n - at : 8);
-    float v[8], r[8];
     const bool whole = VECTOR && count == 8;
+    float v[8], r[8];
     if (whole) {
-      Octet<E>::load(x + at, v);
-      if (RESIDUAL) Octet<E>::load(residual + at, r);
+      Octet<E> c;
+      c.load(x + at);
+      c.unpack(v);
+      if (RESIDUAL) {
+        c.load(residual + at);
+        c.unpack(r);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[i] = i < count ? Octet<E>::get(x + at + i) : 0.f;
-        if (RESIDUAL) r[i] = i < count ? Octet<E>::get(residual + at + i) : 0.f;
+        v[i] = i < count ? element_f32(x[at + i]) : 0.f;
+        r[i] = RESIDUAL && i < count ? element_f32(residual[at + i]) : 0.f;
       }
     }
-    const uint4 bits = philox4x32_10(position + uint64_t(o), keys);
-    const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t field = (i & 1) ? word[i >> 1] >> 16 : word[i >> 1] & 0xffffu;
-      const float kept = field >= threshold ? v[i] * scale : 0.f;
-      v[i] = RESIDUAL ? kept + r[i] : kept;
-    }
+    dropout_octet<RESIDUAL>(v, r, philox4x32_10(position + uint64_t(o), keys), threshold_hi, all, scale);
     if (whole) {
-      Octet<E>::store(y + at, v);
+      Octet<E> c;
+      c.pack(v);
+      c.store(y + at);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i < count) Octet<E>::put(y + at + i, v[i]);
+        if (i < count) element_put(y + at + i, v[i]);
     }
   }
 }
@@ -145,11 +160,14 @@ static int launch_dropout(const void* x, const void* residual, void* y, int64_t 
                           const int64_t* rng, int64_t* rng_used, cudaStream_t st) {
   const bool vec = (((uintptr_t)x | (uintptr_t)y | (uintptr_t)residual) & 15) == 0;
   const int64_t octets = (n + 7) / 8;
-  const unsigned blocks = (unsigned)std::min<int64_t>((octets + 255) / 256, int64_t(sm_count()) * 64);
+  // Blocks that come and go balance the SMs better than eight that stay (16-bit: 64 per SM 193 us, 8 per SM
+  // 208 us, one octet per thread 237 us), fp32, with half the generator's work per byte, the more the better.
+  const int per_sm = sizeof(E) == 4 ? 256 : 64;
+  const unsigned blocks = (unsigned)std::min<int64_t>((octets + 255) / 256, int64_t(sm_count()) * per_sm);
   auto kern = residual != nullptr ? (vec ? dropout_kernel<E, true, true> : dropout_kernel<E, true, false>)
                                   : (vec ? dropout_kernel<E, false, true> : dropout_kernel<E, false, false>);
   kern<<<blocks, 256, 0, st>>>(static_cast<const E*>(x), static_cast<const E*>(residual), static_cast<E*>(y), n,
-                               threshold, scale, rng, rng_used);
+                               threshold << 16, threshold >= 65536u, scale, rng, rng_used);
   PE_LAUNCH_CHECK("dropout_kernel");
   return PE_OK;
 }

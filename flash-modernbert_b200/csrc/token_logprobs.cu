@@ -15,17 +15,21 @@
 // row belongs to one CTA, or, when there are too few rows to fill the GPU, to a cluster of up to
 // eight CTAs that each take a part of the vocabulary and join through distributed shared memory.
 //
-// Top k without a second pass: candidates are pushed into a small shared-memory list as they
-// stream by, if they beat the threshold tau, the k-th best so far.  Order is total: a candidate is the
-// 64-bit number (value's bits made monotone, complement of the index), so equal values
-// rank by lowest index.  When more than 32 threads of a chunk hold a value that beats tau - in the
-// first chunk all do - tau is raised first to the k-th best of the threads' own best, which leaves
-// at most k threads with anything to push; so a chunk adds a bounded number of candidates whatever
-// the data, and the list is cut back to k by counting ranks when it fills up.
+// Top k: the pass also leaves, in shared memory, the largest of every sixteen logits (or multiple of
+// sixteen) that a thread has read.  A threshold follows from them at once: the k / 8-th largest (rounded
+// up) of a warp's 32 thread maxima, the least of these over the eight warps - at least k logits
+// reach it.  Only the sixteens whose largest reaches the threshold are read again, some tens of 3,000 in a
+// row of 50,368, and what reaches the threshold in them is pushed into a small list.  Order is total:
+// a candidate is the 64-bit number (value's bits made monotone, complement of the index), so
+// equal values rank by lowest index.  The list stays bounded whatever the data: when more than 32 threads
+// hold something to push at once, the threshold is raised first to the k-th best of the threads'
+// own best, which leaves at most k of them, and the list is cut back to k by counting ranks when
+// it fills up.
 #include <algorithm>
+#include <type_traits>
 
 #include "pe_host.h"
-#include "pe_ptx.cuh"
+#include "pe_vec.cuh"
 
 #include <cuda_fp16.h>
 
@@ -88,17 +92,25 @@ __device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b) {
   return r;
 }
 
-template <int NT>
+constexpr int LP_TOPS = 16;  // maxima that a thread leaves behind (sixteens are joined beyond 65,536 logits per CTA)
+
+template <int NT, bool TOP>
 struct LpShared {
-  static constexpr int CAP = 1536;  // list of candidates; a chunk adds at most 16 * LP_CROWD = 512
+  static constexpr int CAP = 1536;  // list of candidates; a round adds at most 16 * LP_CROWD = 512
   LpStat stat[NT / 32];
   LpStat part[LP_MAX_CLUSTER];                       // parts of the cluster's CTAs, in rank 0
-  unsigned long long part_top[LP_MAX_CLUSTER * LP_MAX_TOP];
-  unsigned long long best[NT];
-  unsigned long long list[CAP];
-  unsigned long long kept[LP_MAX_TOP];
+  float lse[2];
+  unsigned long long part_top[TOP ? LP_MAX_CLUSTER * LP_MAX_TOP : 1];
+  union {
+    unsigned long long best[TOP ? NT : 1];
+    uint32_t again[TOP ? 2 * NT : 1];                // sixteens to read again: round * NT + thread
+  };
+  unsigned long long list[TOP ? CAP : 1];
+  unsigned long long kept[TOP ? LP_MAX_TOP : 1];
+  float tops[TOP ? LP_TOPS + 1 : 1][TOP ? NT : 1];   // the last row: the odd logits at a row's ends
+  float bound[NT / 32];
   unsigned long long tau;
-  int count;
+  int count, n_again;
 };
 
 // Writes the k best of list[0 .. n) to out[0 .. k) in descending order (0 beyond n).  All threads.
@@ -129,56 +141,72 @@ struct LpArgs {
   int* status;
 };
 
+// Eight or four logits in 16 bytes as fp32.
+template <typename E>
+__device__ __forceinline__ void lp_unpack(const uint4& u, float (&f)[LogitVec<E>::N]) {
+  const E* p = reinterpret_cast<const E*>(&u);
+#pragma unroll
+  for (int i = 0; i < LogitVec<E>::N; ++i) f[i] = logit_f32(p[i]);
+}
+
+// The largest of VECS vectors of logits, NaN if one is: two at a time where the type is packed.
+template <typename E, int VECS>
+__device__ __forceinline__ float lp_top(const uint4 (&u)[VECS]) {
+  if constexpr (sizeof(E) == 4) {
+    float t = __uint_as_float(u[0].x);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+      t = lp_max_nan(lp_max_nan(t, lp_max_nan(__uint_as_float(u[i].x), __uint_as_float(u[i].y))),
+                     lp_max_nan(__uint_as_float(u[i].z), __uint_as_float(u[i].w)));
+    return t;
+  } else {
+    using E2 = typename std::conditional<std::is_same<E, __half>::value, __half2, __nv_bfloat162>::type;
+    E2 t[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const E2* h = reinterpret_cast<const E2*>(&u[i]);
+      t[i] = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    }
+#pragma unroll
+    for (int i = 1; i < VECS; ++i) t[0] = __hmax2_nan(t[0], t[i]);
+    return lp_max_nan(logit_f32(t[0].x), logit_f32(t[0].y));
+  }
+}
+
 template <typename E, int NT, bool TOP>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, TOP ? 4 : 5)
 token_logprobs_kernel(const LpArgs a, int cluster) {
   constexpr int N = LogitVec<E>::N;
-  constexpr int VECS = 16 / N;  // 16-byte loads per thread and chunk: 16 elements
+  constexpr int VECS = 16 / N;  // 16-byte loads per thread and chunk: 16 logits
+  constexpr int CHUNK = NT * VECS;
   constexpr int WARPS = NT / 32;
-  __shared__ LpShared<NT> sh;
+  __shared__ LpShared<NT, TOP> sh;
+  const int tid = threadIdx.x;
   const int rank = cluster > 1 ? int(cluster_ctarank()) : 0;
   const int64_t row = blockIdx.x / cluster;
   const E* x = static_cast<const E*>(a.logits) + row * a.ld;
   const int k = a.top_k;
-  // Vectors are counted from the 16-byte boundary at or below the row's start; those that stick out
-  // of the row (the first and the last at most) are read element by element.
-  const int lead = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(E));
-  const int vecs = (a.vocab + lead + N - 1) / N;
+  // The row in 16-byte vectors from its first 16-byte boundary on; the few logits before that and
+  // behind the last whole vector (`odd` in all, fewer than 2 N) are rank 0's, one to a thread.
+  const int head = min(a.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(E)));
+  const int vecs = (a.vocab - head) / N;
+  const int odd = a.vocab - vecs * N;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   const int per_cta = (vecs + cluster - 1) / cluster;
   const int v_begin = min(vecs, rank * per_cta), v_end = min(vecs, v_begin + per_cta);
+  const int chunks = (v_end - v_begin + CHUNK - 1) / CHUNK;
+  const int join = (chunks + LP_TOPS - 1) / LP_TOPS;  // chunks to a row of sh.tops
+  const int odd_id = rank == 0 && tid < odd ? (tid < head ? tid : vecs * N + tid) : -1;
 
-  auto load = [&](int v, float (&f)[N]) {
-    const int e0 = v * N - lead;
-    if (v < v_end && e0 >= 0 && e0 + N <= a.vocab) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + e0));
-      const E* p = reinterpret_cast<const E*>(&u);
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = logit_f32(p[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        f[i] = v < v_end && e0 + i >= 0 && e0 + i < a.vocab ? logit_f32(x[e0 + i]) : -INFINITY;
-    }
-  };
-
-  if (TOP && threadIdx.x == 0) {
-    sh.tau = 0ull;
-    sh.count = 0;
+  // the row's target, fetched now so that nothing waits for it at the end
+  int64_t target = 0;
+  float x_target = 0.f;
+  if (rank == 0 && tid == 0) {
+    target = a.targets[row];
+    if (target >= 0 && target < a.vocab) x_target = logit_f32(x[target]);
   }
-  if (TOP) __syncthreads();
-
   LpStat st{-INFINITY, 0.f, 0.f};
-  float tau_value = -INFINITY;  // value of sh.tau
-  unsigned long long tau = 0ull;
-  for (int c0 = v_begin; c0 < v_end; c0 += NT * VECS) {
-    float f[VECS][N];
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) load(c0 + i * NT + int(threadIdx.x), f[i]);
-    float top = f[0][0];
-#pragma unroll
-    for (int i = 0; i < VECS; ++i)
-#pragma unroll
-      for (int e = 0; e < N; ++e) top = lp_max_nan(top, f[i][e]);
+  auto raise = [&](float top) {
     if (!(top <= st.m)) {  // a new maximum (or a NaN): move the sums to it
       const float d = st.m == -INFINITY ? 0.f : st.m - top;
       const float z = lp_ex2(d * 1.4426950408889634f);
@@ -186,69 +214,189 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
       st.s *= z;
       st.m = top;
     }
+  };
+  const float2 log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+  float2 s2 = make_float2(0.f, 0.f), w2 = s2;
+  // Whole chunks and one partial, absent vectors as -inf; the next chunk's loads are in flight while
+  // one is worked on.
+  const uint32_t lowest = sizeof(E) == 4 ? 0xff800000u : (std::is_same<E, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
+  uint4 next[VECS];
+  auto load = [&](int v0) {
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = v0 + i * NT + tid;
+      next[i] = v < v_end ? ld_stream(xv + v) : make_uint4(lowest, lowest, lowest, lowest);
+    }
+  };
+  if (chunks > 0) load(v_begin);
+  float joined = -INFINITY;
+  int filled = 0;
+  for (int c = 0; c < chunks; ++c) {
+    const float top = lp_top<E, VECS>(next);
+    float f[VECS][N];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) lp_unpack<E>(next[i], f[i]);
+    if (c + 1 < chunks) load(v_begin + (c + 1) * CHUNK);
+    if (TOP) {
+      joined = lp_max_nan(joined, top);
+      if (++filled == join || c + 1 == chunks) {
+        sh.tops[c / join][tid] = joined;
+        joined = -INFINITY;
+        filled = 0;
+      }
+    }
+    if (!(top <= st.m)) {
+      st.s += s2.x + s2.y;
+      st.w += w2.x + w2.y;
+      s2 = w2 = make_float2(0.f, 0.f);
+      raise(top);
+    }
     const float ref = st.m == -INFINITY ? 0.f : st.m;
+    const float2 neg_ref = make_float2(-ref, -ref);
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float d = f[i][e] - ref;
-        const float p = lp_ex2(d * 1.4426950408889634f);
-        st.s += p;
-        st.w = fmaf(p, fmaxf(d, -3.0e38f), st.w);  // 0 * -inf would be NaN
+      for (int e = 0; e < N; e += 2) {
+        float2 d = __fadd2_rn(make_float2(f[i][e], f[i][e + 1]), neg_ref);
+        const float2 y = __fmul2_rn(d, log2e);
+        const float2 q = make_float2(lp_ex2(y.x), lp_ex2(y.y));
+        d = make_float2(fmaxf(d.x, -3.0e38f), fmaxf(d.y, -3.0e38f));  // 0 * -inf would be NaN
+        s2 = __fadd2_rn(s2, q);
+        w2 = __ffma2_rn(q, d, w2);
       }
-    if (TOP) {
-      // the best of this thread's sixteen that beats tau
-      unsigned long long best = 0ull;
-      if (!(top < tau_value)) {
-#pragma unroll
-        for (int i = 0; i < VECS; ++i)
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const int id = (c0 + i * NT + int(threadIdx.x)) * N - lead + e;
-            const bool real = id >= 0 && id < a.vocab && c0 + i * NT + int(threadIdx.x) < v_end;
-            const unsigned long long key = real ? lp_key(f[i][e], uint32_t(id)) : 0ull;
-            if (key > tau && key > best) best = key;
-          }
+  }
+  st.s += s2.x + s2.y;
+  st.w += w2.x + w2.y;
+  if (odd_id >= 0) {
+    const float v = logit_f32(x[odd_id]);
+    raise(v);
+    const float ref = st.m == -INFINITY ? 0.f : st.m;
+    const float d = v - ref, q = lp_ex2(d * 1.4426950408889634f);
+    st.s += q;
+    st.w = fmaf(q, fmaxf(d, -3.0e38f), st.w);
+    if (TOP) sh.tops[LP_TOPS][tid] = v;
+  }
+
+  if (TOP) {
+    // Threshold: from the warps whose lanes all have logits, so that at least k reach it (none: 0).
+    const int full_warps = min(WARPS, (v_end - v_begin) / 32);
+    {
+      const int lane = tid & 31;
+      uint32_t mine = uint32_t(lp_key(st.m, 0) >> 32), level = 0u;
+      for (int taken = 0; taken < k; taken += full_warps == 0 ? k : full_warps) {
+        level = __reduce_max_sync(0xffffffffu, mine);
+        const uint32_t holders = __ballot_sync(0xffffffffu, mine == level);
+        if (lane == __ffs(holders) - 1) mine = 0u;
       }
-      const int holders = __syncthreads_count(best != 0ull);
-      if (holders > 0) {
-        if (holders > LP_CROWD) {
-          sh.best[threadIdx.x] = best;
-          __syncthreads();
-          if (best != 0ull) {
-            int above = 0;
-            for (int j = 0; j < NT; ++j) above += sh.best[j] > best;
-            if (above == k - 1) sh.tau = best - 1;  // everything from the k-th best on may push
+      if (lane == 0) sh.bound[tid >> 5] = __uint_as_float(level);
+    }
+    if (tid == 0) sh.count = sh.n_again = 0;
+    __syncthreads();
+    uint32_t level = full_warps == 0 ? 0u : 0xffffffffu;
+    for (int i = 0; i < full_warps; ++i) level = min(level, __float_as_uint(sh.bound[i]));
+    // what equals the threshold may be pushed too
+    unsigned long long tau = level == 0u ? 0ull : (static_cast<unsigned long long>(level) << 32) - 1ull;
+    // The usual way: list the sixteens that reach tau, then read them all at once, one to a thread.
+    for (int r = 0; r < chunks; ++r)
+      if (v_begin + r * CHUNK + tid < v_end && lp_key(sh.tops[r / join][tid], 0u) > tau) {
+        const int at = atomicAdd(&sh.n_again, 1);
+        if (at < 2 * NT) sh.again[at] = uint32_t(r) * NT + tid;
+      }
+    auto push = [&](unsigned long long key) {
+      if (key > tau) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < LpShared<NT, TOP>::CAP) sh.list[at] = key;
+      }
+    };
+    if (odd_id >= 0) push(lp_key(logit_f32(x[odd_id]), uint32_t(odd_id)));
+    __syncthreads();
+    const int n_again = sh.n_again;
+    if (n_again <= 2 * NT) {
+      for (int i = tid; i < n_again; i += NT) {
+        const int r = sh.again[i] / NT, v0 = v_begin + r * CHUNK + int(sh.again[i] % NT);
+        uint4 u[VECS];
+#pragma unroll
+        for (int q = 0; q < VECS; ++q) u[q] = v0 + q * NT < v_end ? __ldg(xv + v0 + q * NT) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int q = 0; q < VECS; ++q) {
+          float f[N];
+          lp_unpack<E>(u[q], f);
+          if (v0 + q * NT < v_end) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) push(lp_key(f[e], uint32_t(head + (v0 + q * NT) * N + e)));
           }
-          __syncthreads();
-          tau = sh.tau;
         }
-        if (best > tau) {
+      }
+    }
+    __syncthreads();
+    const bool crowded = n_again > 2 * NT || sh.count > LpShared<NT, TOP>::CAP;  // the same for every thread
+    __syncthreads();
+    if (crowded && tid == 0) sh.count = 0;
+    __syncthreads();
+    // Otherwise, whatever the data, in rounds of bounded size.
+    // Round r < chunks: sixteen logits of every thread whose maximum is not below tau; the last round:
+    // the odd ones.
+    for (int r = 0; crowded && r <= chunks; ++r) {
+      const bool ends = r == chunks;
+      const int v0 = v_begin + r * CHUNK + tid;  // its vectors: v0, v0 + NT, ...
+      bool flag = ends ? odd_id >= 0 : v0 < v_end;
+      if (flag) flag = lp_key(sh.tops[ends ? LP_TOPS : r / join][tid], 0u) > tau;
+      const int flagged = __syncthreads_count(flag);
+      if (flagged == 0) continue;
+      float f[VECS][N];
+      if (flag) {
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+          if (!ends && v0 + i * NT < v_end) lp_unpack<E>(__ldg(xv + v0 + i * NT), f[i]);
+        }
+        if (ends) f[0][0] = logit_f32(x[odd_id]);
+      }
+      auto key_of = [&](int i, int e) {  // 0: not there
+        if (ends) return i == 0 && e == 0 ? lp_key(f[0][0], uint32_t(odd_id)) : 0ull;
+        return v0 + i * NT < v_end ? lp_key(f[i][e], uint32_t(head + (v0 + i * NT) * N + e)) : 0ull;
+      };
+      if (flagged > LP_CROWD) {
+        unsigned long long best = 0ull;
+        if (flag) {
 #pragma unroll
           for (int i = 0; i < VECS; ++i)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-              const int id = (c0 + i * NT + int(threadIdx.x)) * N - lead + e;
-              const bool real = id >= 0 && id < a.vocab && c0 + i * NT + int(threadIdx.x) < v_end;
-              const unsigned long long key = real ? lp_key(f[i][e], uint32_t(id)) : 0ull;
-              if (key > tau) sh.list[atomicAdd(&sh.count, 1)] = key;
+              const unsigned long long key = key_of(i, e);
+              best = key > best ? key : best;
             }
+          if (best <= tau) best = 0ull;
+        }
+        sh.best[tid] = best;
+        if (tid == 0) sh.tau = tau;
+        __syncthreads();
+        if (best != 0ull) {
+          int above = 0;
+          for (int j = 0; j < NT; ++j) above += sh.best[j] > best;
+          if (above == k - 1) sh.tau = best - 1ull;  // everything from the k-th best on may push
         }
         __syncthreads();
-        const int n = sh.count;
-        if (n > LpShared<NT>::CAP - 16 * LP_CROWD) {  // the next chunk might not fit: keep the k best
-          lp_select<NT>(sh.list, n, k, sh.kept);
-          __syncthreads();
-          for (int i = threadIdx.x; i < k; i += NT) sh.list[i] = sh.kept[i];
-          if (threadIdx.x == 0) {
-            sh.count = k;
-            sh.tau = sh.kept[k - 1];
+        tau = sh.tau;
+        flag = flag && best > tau;
+      }
+      if (flag) {
+#pragma unroll
+        for (int i = 0; i < VECS; ++i)
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const unsigned long long key = key_of(i, e);
+            if (key > tau) sh.list[atomicAdd(&sh.count, 1)] = key;
           }
-          __syncthreads();
-          tau = sh.tau;
-        }
-        tau_value = tau != 0ull ? lp_key_value(tau) : -INFINITY;
-        if (tau_value != tau_value) tau_value = INFINITY;  // only NaN can still beat a NaN: none does by value
+      }
+      __syncthreads();
+      const int n = sh.count;
+      if (n > LpShared<NT, TOP>::CAP - 16 * LP_CROWD) {  // the next round might not fit: keep the k best
+        lp_select<NT>(sh.list, n, k, sh.kept);
+        __syncthreads();
+        for (int i = tid; i < k; i += NT) sh.list[i] = sh.kept[i];
+        if (tid == 0) sh.count = k;
+        tau = sh.kept[k - 1];
+        __syncthreads();
       }
     }
   }
@@ -265,9 +413,16 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
   if ((threadIdx.x & 31) == 0) sh.stat[threadIdx.x >> 5] = st;
   __syncthreads();
   if (TOP) lp_select<NT>(sh.list, sh.count, k, sh.kept);
-  if (threadIdx.x == 0) {
-    st = sh.stat[0];
-    for (int i = 1; i < WARPS; ++i) st = lp_join(st, sh.stat[i]);
+  if (threadIdx.x < 32) {
+    st = threadIdx.x < WARPS ? sh.stat[threadIdx.x] : LpStat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) {
+      LpStat other;
+      other.m = __shfl_down_sync(0xffffffffu, st.m, o);
+      other.s = __shfl_down_sync(0xffffffffu, st.s, o);
+      other.w = __shfl_down_sync(0xffffffffu, st.w, o);
+      st = lp_join(st, other);
+    }
   }
   if (cluster > 1) {
     __syncthreads();
@@ -300,20 +455,19 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
     a.lse[row] = lse;
     a.lse_rest[row] = rest;
     a.entropy[row] = log_s - st.w / st.s;
-    const int64_t t = a.targets[row];
     float lp = 0.f;
-    if (t >= 0 && t < a.vocab) lp = t == a.ignore_index ? 0.f : (logit_f32(x[t]) - lse) - rest;
-    else if (t != a.ignore_index) set_status(a.status, ST_BAD_TARGET);
+    if (target >= 0 && target < a.vocab) lp = target == a.ignore_index ? 0.f : (x_target - lse) - rest;
+    else if (target != a.ignore_index) set_status(a.status, ST_BAD_TARGET);
     a.logprobs[row] = lp;
-    sh.stat[0].m = lse;
-    sh.stat[0].s = rest;
+    sh.lse[0] = lse;
+    sh.lse[1] = rest;
   }
   if (TOP) {
     __syncthreads();
     if (threadIdx.x < k) {
       const unsigned long long key = sh.kept[threadIdx.x];
       a.top_ids[row * k + threadIdx.x] = int64_t(0xffffffffu - uint32_t(key));
-      a.top_logprobs[row * k + threadIdx.x] = (lp_key_value(key) - sh.stat[0].m) - sh.stat[0].s;
+      a.top_logprobs[row * k + threadIdx.x] = (lp_key_value(key) - sh.lse[0]) - sh.lse[1];
     }
   }
 }
@@ -334,53 +488,99 @@ struct LpBackArgs {
   int vocab;
 };
 
-// Grid (chunks of the vocabulary, rows).  VECTOR: input and output rows lie alike relative to
-// 16-byte boundaries, so a thread moves 16 bytes at a time.
+// Grid (parts of the vocabulary, rows); a block walks its part, the loads of its next step in flight while it
+// works on one.  VECTOR: input and output rows lie alike relative to 16-byte boundaries, so a piece
+// is 16 bytes, else one logit.  A row whose three gradients are zero (an ignored target) is not read.
+constexpr int LP_BACK = 2;  // pieces per thread and step
+
+__device__ __forceinline__ void lp_pack(uint4& u, const float (&f)[8], __nv_bfloat16) { u = pack8(f); }
+__device__ __forceinline__ void lp_pack(uint4& u, const float (&f)[8], __half) {
+  __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ void lp_pack(uint4& u, const float (&f)[4], float) {
+  u = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+
 template <typename E, bool VECTOR>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
 token_logprobs_backward_kernel(const LpBackArgs a, int64_t rows) {
   constexpr int N = VECTOR ? LogitVec<E>::N : 1;
+  constexpr int LANES = LogitVec<E>::N;  // of a register vector, of which !VECTOR uses the first
+  constexpr int STEP = 256 * LP_BACK;
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     const E* x = static_cast<const E*>(a.logits) + row * a.ld;
     E* dx = static_cast<E*>(a.dlogits) + row * a.ld_out;
+    const int lead = VECTOR ? int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(E)) : 0;
+    const int vecs = (a.vocab + lead + N - 1) / N;  // the first and the last may stick out of the row
+    const int steps = (vecs + STEP - 1) / STEP, per_part = (steps + int(gridDim.x) - 1) / int(gridDim.x);
+    const int s_end = min(steps, (int(blockIdx.x) + 1) * per_part);
+    int s = int(blockIdx.x) * per_part;
+    if (s >= s_end) continue;
     const int64_t t = a.targets[row];
     const bool kept = t >= 0 && t < a.vocab && t != a.ignore_index;
     const float g = kept && a.d_logprobs != nullptr ? a.d_logprobs[row] : 0.f;
     const float h = a.d_entropy != nullptr ? a.d_entropy[row] : 0.f;
     const float z = a.d_lse != nullptr ? a.d_lse[row] : 0.f;
-    const bool nothing = g == 0.f && h == 0.f && z == 0.f;  // an ignored row: zeros, nothing read
     const float lse = a.lse[row], rest = a.lse_rest[row], ent = a.entropy[row];
-    const int lead = VECTOR ? int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(E)) : 0;
-    const int vecs = (a.vocab + lead + N - 1) / N;
-    for (int v = blockIdx.x * blockDim.x + threadIdx.x; v < vecs; v += gridDim.x * blockDim.x) {
-      const int e0 = v * N - lead;
-      const bool whole = e0 >= 0 && e0 + N <= a.vocab;
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      E* q = reinterpret_cast<E*>(&u);
-      if (!nothing) {
-        if (VECTOR && whole) {
-          u = *reinterpret_cast<const uint4*>(x + e0);
+    const bool nothing = g == 0.f && h == 0.f && z == 0.f;
+    const float zg = z - g;
+    // p (z - g - h (log p + H)) of one logit; log p is kept finite, so a token of probability zero has
+    // no part in the entropy's gradient
+    auto gradient = [&](float v) {
+      const float lp = (v - lse) - rest;
+      return lp_ex2(lp * 1.4426950408889634f) * fmaf(-h, fmaxf(lp, -1.0e30f) + ent, zg);
+    };
+    auto whole = [&](int v) { return VECTOR && v * N >= lead && v * N - lead + N <= a.vocab; };
+    uint4 next[LP_BACK];
+    auto load = [&](int step) {
+#pragma unroll
+      for (int i = 0; i < LP_BACK; ++i) {
+        next[i] = make_uint4(0u, 0u, 0u, 0u);
+        const int v = step * STEP + i * 256 + int(threadIdx.x), e0 = v * N - lead;
+        if (nothing || v >= vecs) continue;
+        if (whole(v)) {
+          next[i] = *reinterpret_cast<const uint4*>(x + e0);
         } else {
 #pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (e0 + i >= 0 && e0 + i < a.vocab) q[i] = x[e0 + i];
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float lp = (logit_f32(q[i]) - lse) - rest;
-          const float p = lp_ex2(lp * 1.4426950408889634f);
-          // p (z - g - h (log p + H)); a token of probability zero has no part in the entropy
-          float d = p * (z - g - (p == 0.f ? 0.f : h * (lp + ent)));
-          if (e0 + i == t) d += g;
-          logit_put(q + i, d);
+          for (int e = 0; e < N; ++e)
+            if (e0 + e >= 0 && e0 + e < a.vocab) reinterpret_cast<E*>(&next[i])[e] = x[e0 + e];
         }
       }
-      if (VECTOR && whole) {
-        *reinterpret_cast<uint4*>(dx + e0) = u;
-      } else {
+    };
+    load(s);
+    for (; s < s_end; ++s) {
+      uint4 u[LP_BACK];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (e0 + i >= 0 && e0 + i < a.vocab) dx[e0 + i] = q[i];
+      for (int i = 0; i < LP_BACK; ++i) u[i] = next[i];
+      if (s + 1 < s_end) load(s + 1);
+#pragma unroll
+      for (int i = 0; i < LP_BACK; ++i) {
+        const int v = s * STEP + i * 256 + int(threadIdx.x), e0 = v * N - lead;
+        if (v >= vecs) break;
+        const bool mine = !nothing && t >= e0 && t < e0 + N;  // the target is among these
+        float at_target = 0.f;
+        if (!nothing) {
+          float f[LANES];
+          lp_unpack<E>(u[i], f);
+          if (mine) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (e0 + e == t) at_target = gradient(f[e]) + g;
+          }
+#pragma unroll
+          for (int e = 0; e < N; ++e) f[e] = gradient(f[e]);
+          lp_pack(u[i], f, E());
+        }
+        if (whole(v)) {
+          *reinterpret_cast<uint4*>(dx + e0) = u[i];
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (e0 + e >= 0 && e0 + e < a.vocab) dx[e0 + e] = reinterpret_cast<const E*>(&u[i])[e];
+        }
+        if (mine) logit_put(dx + t, at_target);
       }
     }
   }
@@ -415,8 +615,12 @@ static int launch_logprobs_backward(const LpBackArgs& a, int64_t rows, cudaStrea
   const bool alike = ((uintptr_t)a.logits & 15) == ((uintptr_t)a.dlogits & 15) &&
                      (a.ld - a.ld_out) * int64_t(sizeof(E)) % 16 == 0;
   const int per_thread = alike ? LogitVec<E>::N : 1;
-  const int64_t chunks = (a.vocab + int64_t(256) * per_thread * 4 - 1) / (int64_t(256) * per_thread * 4);
-  const dim3 grid((unsigned)chunks, (unsigned)std::min<int64_t>(rows, 65535));
+  // A row to a block as long as there are enough of them to keep every SM's five blocks busy for a few
+  // turns, else parts of a row, down to one step (4,096 logits of 16 bits) each.
+  const int64_t per_step = int64_t(256) * LP_BACK * per_thread;
+  const int64_t steps = (a.vocab + (per_thread - 1) + per_step - 1) / per_step;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(steps, int64_t(sm_count()) * 20 / rows));
+  const dim3 grid((unsigned)parts, (unsigned)std::min<int64_t>(rows, 65535));
   auto kern = alike ? token_logprobs_backward_kernel<E, true> : token_logprobs_backward_kernel<E, false>;
   kern<<<grid, 256, 0, st>>>(a, rows);
   PE_LAUNCH_CHECK("token_logprobs_backward_kernel");

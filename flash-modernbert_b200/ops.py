@@ -41,18 +41,22 @@ def _index_cuda(t: Tensor, name: str, dtype: torch.dtype, like: Tensor) -> Tenso
 class _Call:
     """Device guard + stream + status word for one library call."""
 
+    __slots__ = ("lib", "index", "guard", "stream")
+
     def __init__(self, ref: Tensor):
         self.lib = _lib.load()
-        self.device = ref.device
-        self.guard = torch.cuda.device(self.device)
+        self.index = ref.device.index
+        # switching to the device that is current already costs more than the launch of a small kernel
+        self.guard = None if torch.cuda.current_device() == self.index else torch.cuda.device(self.index)
 
     def __enter__(self):
-        self.guard.__enter__()
-        self.stream = _lib.current_stream_ptr()
+        if self.guard is not None:
+            self.guard.__enter__()
+        self.stream = _lib.device_stream_ptr(self.index)
         return self
 
     def __exit__(self, *exc):
-        return self.guard.__exit__(*exc)
+        return None if self.guard is None else self.guard.__exit__(*exc)
 
 
 _status_words: dict[int, Tensor] = {}
@@ -521,14 +525,17 @@ def _targets_for(targets: Tensor, logits: Tensor) -> Tensor:
     return targets.reshape(-1)
 
 
-def _logprobs_call(logits: Tensor, targets: Tensor, top_k: int, ignore_index: int) -> TokenLogprobs:
+def _logprobs_call(logits: Tensor, targets: Tensor, top_k: int, ignore_index: int, separate: bool) -> TokenLogprobs:
     rows, ld = _logit_rows(logits, "logits")
     flat = _targets_for(targets, logits)
     vocab, lead = rows.shape[1], logits.shape[:-1]
     if not 0 <= top_k <= min(32, vocab):
         raise ValueError(f"top_k must be within 0..{min(32, vocab)}, got {top_k}")
     n, dev = rows.shape[0], logits.device
-    stats = [torch.empty(n, dtype=torch.float32, device=dev) for _ in range(4)]
+    if separate:  # outputs of an autograd function that the caller may change in place
+        stats = [torch.empty(n, dtype=torch.float32, device=dev) for _ in range(4)]
+    else:
+        stats = torch.empty(4, n, dtype=torch.float32, device=dev).unbind(0)
     ids = torch.empty(n, top_k, dtype=torch.int64, device=dev) if top_k else None
     top = torch.empty(n, top_k, dtype=torch.float32, device=dev) if top_k else None
     with _Call(logits) as c:
@@ -536,14 +543,16 @@ def _logprobs_call(logits: Tensor, targets: Tensor, top_k: int, ignore_index: in
                                            int(ignore_index), top_k, stats[0].data_ptr(), stats[1].data_ptr(),
                                            stats[2].data_ptr(), stats[3].data_ptr(), _lib.ptr(ids), _lib.ptr(top),
                                            status_word(dev).data_ptr(), c.stream), "pe_token_logprobs")
-    shaped = [s.view(lead) for s in stats]
-    return TokenLogprobs(*shaped, *((t.view(*lead, top_k) if top_k else None) for t in (ids, top)))
+    if len(lead) != 1:
+        stats = [s.view(lead) for s in stats]
+        ids, top = ((t.view(*lead, top_k) if top_k else None) for t in (ids, top))
+    return TokenLogprobs(*stats, ids, top)
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, ignore_index):
-        r = _logprobs_call(logits, targets, top_k, ignore_index)
+        r = _logprobs_call(logits, targets, top_k, ignore_index, True)
         ctx.save_for_backward(logits, targets, r.lse, r.lse_rest, r.entropy)
         ctx.ignore_index = ignore_index
         ctx.set_materialize_grads(False)
@@ -569,7 +578,7 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, top_k: int = 0, ignore_in
     probability 0. Differentiable through `logprobs`, `entropy` and `lse`, not through the top."""
     if torch.is_grad_enabled() and isinstance(logits, Tensor) and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, int(top_k), int(ignore_index)))
-    return _logprobs_call(logits, targets, int(top_k), int(ignore_index))
+    return _logprobs_call(logits, targets, int(top_k), int(ignore_index), False)
 
 
 def token_logprobs_backward(logits: Tensor, targets: Tensor, forward: TokenLogprobs, d_logprobs: Tensor | None,
