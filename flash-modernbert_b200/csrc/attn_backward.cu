@@ -38,48 +38,47 @@ namespace pe {
 // Three groups of four compute warps take a row tile's column tiles in turn; each is a chain of tensor
 // memory loads, exponentials, stores and barrier round trips that no group could hide alone, and
 // three of them fill each other's gaps.  A column tile is 64 wide so that each group can own the two
-// 64-column buffers it needs beside the accumulators.
+// 64-column buffers it needs beside the accumulators.  Four more warps move finished accumulators out: a
+// group that did it itself was away from its next tiles for some 4,000 clocks per item (307,164
+// tokens x 12 heads, window 64: 2.01 ms against 1.43 ms).
 constexpr int BW_GROUPS = 3;
 constexpr int BW_COMPUTE_WARPS = 4 * BW_GROUPS;
 constexpr int BW_PRODUCER = BW_COMPUTE_WARPS;
 constexpr int BW_MMA = BW_COMPUTE_WARPS + 1;
-constexpr int BW_THREADS = 32 * (BW_COMPUTE_WARPS + 2);
+constexpr int BW_STORER = BW_COMPUTE_WARPS + 4;       // first of four (two in between idle: registers move by fours)
+constexpr int BW_THREADS = 32 * (BW_COMPUTE_WARPS + 8);
 constexpr int BW_TILE = 128;                        // rows of a row tile
 constexpr int BW_COLS = 64;                         // columns of a column tile
 constexpr int BW_A_BYTES = BW_TILE * 64 * 2;        // one operand of a row tile
 constexpr int BW_B_BYTES = BW_COLS * 64 * 2;        // one operand of a column tile
-// The g-th column tile of a CTA belongs to group g % 3 and uses slot g % 6 of everything: the operand
-// ring in shared memory ((Q, dO) or (K, V), lse and delta), tensor memory and the barriers, whose
-// phases therefore all count g / 6.
+// The g-th column tile of a CTA belongs to group w = g % 3 and uses slot 2 w + g / 3 % 2 of everything: the
+// operand ring in shared memory ((Q, dO) or (K, V), lse and delta), tensor memory and the barriers,
+// whose phases therefore all count g / 6.
 constexpr int BW_SLOTS = 2 * BW_GROUPS;
 constexpr int BW_STATS_BYTES = 2 * BW_COLS * 4;     // lse and delta of a column tile
-constexpr int BW_OUT_BYTES = 32 * 128;              // a compute warp's 32 rows of one gradient on their way out
+constexpr int BW_OUT_BYTES = 2 * 32 * 128;          // 32 rows of both gradients on their way out
 constexpr uint32_t BW_TMEM_COLS = 512;
-// Tensor memory: slots w and w + 3 are group w's two buffers of 64 columns, at 128 w and 64 further on.
-// The scores of a tile go to its own slot's buffer, dP to the group's other one.  The scores are
-// replaced in place by P (32 columns of bf16 pairs) and dS (32 more).  Once dP has been read its
-// buffer takes the group's next scores; once P and dS have been multiplied theirs takes the next dP.
-constexpr uint32_t BW_ACC1_COL = 384;  // dK or dQ
-constexpr uint32_t BW_ACC2_COL = 448;  // dV
+// Tensor memory: a buffer of 64 columns per slot, at 64 c.  The scores of a tile go to its own slot's buffer,
+// dP to the group's other one (c ^ 1).  The scores are replaced in place by P (32 columns of bf16
+// pairs) and dS (32 more).  Once dP has been read its buffer takes the group's next scores; once P
+// and dS have been multiplied theirs takes the next dP.
+constexpr uint32_t BW_ACC1_COL = 384;  // dK; dQ of even items
+constexpr uint32_t BW_ACC2_COL = 448;  // dV; dQ of odd items
 
 // Barriers of one pass; each pass has its own set.  [c]: one per slot.
 enum {
-  WB_FULL = 0,                          // [c]
-  WB_EMPTY = WB_FULL + BW_SLOTS,        // [c]
-  WB_S_FULL = WB_EMPTY + BW_SLOTS,      // [c]
+  WB_IN = 0,                            // [c] the tile's operands are here and dS of the tile three before it is written
+  WB_S_FULL = WB_IN + BW_SLOTS,         // [c]
   WB_DP_FULL = WB_S_FULL + BW_SLOTS,    // [c]
-  WB_DK_DONE = WB_DP_FULL + BW_SLOTS,   // [c] the tile's dK (or dQ) has retired, and all issued before it
-  WB_A_FULL = WB_DK_DONE + BW_SLOTS,    // [2]
+  WB_DONE = WB_DP_FULL + BW_SLOTS,      // [c] the tile has been accumulated
+  WB_A_FULL = WB_DONE + BW_SLOTS,       // [2]
   WB_A_EMPTY = WB_A_FULL + 2,           // [2]
-  // from here on: one arrival per warp of a group
-  WB_P_FULL = WB_A_EMPTY + 2,           // [c] P written (key pass)
-  WB_DP_READ = WB_P_FULL + BW_SLOTS,    // [c]
-  WB_DS_FULL = WB_DP_READ + BW_SLOTS,   // [c]
-  WB_ACC_EMPTY = WB_DS_FULL + BW_SLOTS, // the item's accumulators have been read
-  WB_COUNT = WB_ACC_EMPTY + 1
+  WB_ACC_FULL = WB_A_EMPTY + 2,         // [2]
+  WB_ACC_EMPTY = WB_ACC_FULL + 2,       // [2] the item's accumulators have been read
+  WB_COUNT = WB_ACC_EMPTY + 2
 };
 constexpr int BW_OUT_OFFSET = 4 * BW_A_BYTES + BW_SLOTS * 2 * BW_B_BYTES;
-constexpr int BW_STATS_OFFSET = BW_OUT_OFFSET + BW_COMPUTE_WARPS * BW_OUT_BYTES;
+constexpr int BW_STATS_OFFSET = BW_OUT_OFFSET + 4 * BW_OUT_BYTES;
 constexpr int BW_BAR_OFFSET = BW_STATS_OFFSET + BW_SLOTS * BW_STATS_BYTES;
 constexpr int BW_SMEM = BW_BAR_OFFSET + 2 * WB_COUNT * 8 + 16;
 static_assert(BW_SMEM <= 227 * 1024, "shared memory of one CTA");
@@ -219,6 +218,96 @@ struct BwItem {
   __device__ __forceinline__ int col0(int j) const { return j + 1 == n ? hi - BW_COLS : lo + j * BW_COLS; }
 };
 
+// A waiting instruction takes about a hundred clocks to answer even when its phase is complete.  This one does
+// not wait: it is issued ahead of other work, and only where its answer, read after that work, is "not
+// yet" does a wait follow.
+__device__ __forceinline__ bool bw_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Bounded: the instruction itself waits up to about half a microsecond, so this gives up after seconds at most.
+__device__ __forceinline__ bool bw_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 0;\n\t"
+      "WAIT:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+      "@P bra DONE;\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.lt.u32 P, n, 4194304;\n\t"
+      "@P bra WAIT;\n\t"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(500u)
+      : "memory");
+  return done != 0;
+}
+// Four products over 16 of 64 dimensions each (or columns, below), an arrival on `commit` when all issued so far
+// have retired, and the state of another barrier, which is asked for before and read after: the answer
+// takes about as long as the products take to be accepted.
+__device__ __forceinline__ bool bw_products_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                               uint32_t commit, uint32_t test, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred T, P, Q;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 T, [%7], %8;\n\t"
+      "setp.ne.b32 P, %1, %1;\n\t"
+      "setp.eq.b32 Q, %1, %1;\n\t"
+      "mov.b64 a, {%2, %4};\n\tmov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %5, P;\n\t"
+      "add.u32 x, %2, 2;\n\tadd.u32 y, %3, 2;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %5, Q;\n\t"
+      "add.u32 x, %2, 4;\n\tadd.u32 y, %3, 4;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %5, Q;\n\t"
+      "add.u32 x, %2, 6;\n\tadd.u32 y, %3, 6;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %5, Q;\n\t"
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t"
+      "selp.u32 %0, 1, 0, T;\n\t}\n"
+      : "=r"(done)
+      : "r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(commit), "r"(test), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// A in tensor memory (64 columns as pairs), B's rows 2048 bytes (descriptor units of 16) further on each time.
+__device__ __forceinline__ bool bw_products_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                               uint32_t add, uint32_t commit, uint32_t test, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred T, P, Q;\n\t.reg .b64 b;\n\t.reg .b32 x, y;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 T, [%8], %9;\n\t"
+      "setp.ne.b32 P, %6, 0;\n\t"
+      "setp.eq.b32 Q, %1, %1;\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], b, %5, P;\n\t"
+      "add.u32 x, %2, 8;\n\tadd.u32 y, %3, 128;\n\tmov.b64 b, {y, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], [x], b, %5, Q;\n\t"
+      "add.u32 x, %2, 16;\n\tadd.u32 y, %3, 256;\n\tmov.b64 b, {y, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], [x], b, %5, Q;\n\t"
+      "add.u32 x, %2, 24;\n\tadd.u32 y, %3, 384;\n\tmov.b64 b, {y, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%1], [x], b, %5, Q;\n\t"
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t"
+      "selp.u32 %0, 1, 0, T;\n\t}\n"
+      : "=r"(done)
+      : "r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(add), "r"(commit), "r"(test), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Slot of the tile after the one in slot c: 0, 2, 4, 1, 3, 5, 0, ...
+__device__ __forceinline__ uint32_t bw_next_slot(uint32_t c) { return c + 2 < BW_SLOTS ? c + 2 : BW_SLOTS + 1 - (c + 2); }
+// Bits [lo, hi) of a word.
+__device__ __forceinline__ uint32_t bw_bits(int lo, int hi) {
+  const uint32_t below_hi = hi >= 32 ? 0xffffffffu : (1u << max(hi, 0)) - 1u;
+  return lo >= 32 ? 0u : below_hi & ~((1u << max(lo, 0)) - 1u);
+}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -233,10 +322,12 @@ __device__ __forceinline__ float4 lds128(uint32_t addr) {
   return v;
 }
 
-// 64 accumulated values of a row, scaled, as 32 bf16 pairs; with `trow` (the rotation table's row of the
-// row's position) the rotation is undone first: the transpose of what was applied to q and k.
-__device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, const uint4* trow, uint32_t (&out)[32]) {
-#pragma unroll
+// 64 accumulated values of a row, scaled, as bf16 to the warp's block of shared memory, a row of 128 bytes per
+// thread; zeros if the row attends nothing.  With `trow` (the rotation table's row of the row's position) the
+// rotation is undone first: the transpose of what was applied to q and k.
+__device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, const uint4* trow, bool empty,
+                                              uint32_t block, int lane) {
+#pragma unroll 1
   for (int c = 0; c < 2; ++c) {  // dimensions [16 c, 16 c + 16) and those they are paired with, 32 further on
     uint32_t lo[16], hi[16];
     g_tmem_ld16(acc_addr + c * 16, lo);
@@ -247,8 +338,8 @@ __device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, co
       float x[8], y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = __uint_as_float(lo[h * 8 + e]) * scale;
-        y[e] = __uint_as_float(hi[h * 8 + e]) * scale;
+        x[e] = empty ? 0.f : __uint_as_float(lo[h * 8 + e]) * scale;
+        y[e] = empty ? 0.f : __uint_as_float(hi[h * 8 + e]) * scale;
       }
       if (trow != nullptr) {
         float cs[8], sn[8];
@@ -261,27 +352,22 @@ __device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, co
           y[e] = fmaf(w, cs[e], -(u * sn[e]));
         }
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        out[c * 8 + h * 4 + e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-        out[16 + c * 8 + h * 4 + e] = pack_bf16(y[2 * e], y[2 * e + 1]);
-      }
+      const int i = c * 2 + h;  // 16-byte chunk of the row
+      const uint32_t row = block + lane * 128;
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((i ^ (lane & 7)) << 4)),
+                   "r"(pack_bf16(x[0], x[1])), "r"(pack_bf16(x[2], x[3])), "r"(pack_bf16(x[4], x[5])),
+                   "r"(pack_bf16(x[6], x[7]))
+                   : "memory");
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((i + 4) ^ (lane & 7)) << 4)),
+                   "r"(pack_bf16(y[0], y[1])), "r"(pack_bf16(y[2], y[3])), "r"(pack_bf16(y[4], y[5])),
+                   "r"(pack_bf16(y[6], y[7]))
+                   : "memory");
     }
   }
 }
-// Stores a warp's 32 rows of 64 bf16 values, a row per thread (zeros if it is empty): turned in the warp's
-// own block of shared memory, so that an instruction writes four whole 128-byte rows.  `dst` is the
-// first row's, `rows` how many of them exist.
-__device__ __forceinline__ void bw_store_rows(__nv_bfloat16* dst, int64_t ld, int rows, uint32_t block, int lane,
-                                              const uint32_t (&v)[32], bool empty) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(block + lane * 128 + ((i ^ (lane & 7)) << 4)),
-                 "r"(empty ? 0u : v[4 * i]), "r"(empty ? 0u : v[4 * i + 1]), "r"(empty ? 0u : v[4 * i + 2]),
-                 "r"(empty ? 0u : v[4 * i + 3])
-                 : "memory");
-  __syncwarp();
-#pragma unroll
+// The block's rows to memory, four whole rows per instruction; `dst` is the first row's, `rows` how many of them exist.
+__device__ __forceinline__ void bw_store_rows(__nv_bfloat16* dst, int64_t ld, int rows, uint32_t block, int lane) {
+#pragma unroll 4
   for (int i = 0; i < 8; ++i) {
     const int r = i * 4 + (lane >> 3);
     uint4 u;
@@ -291,12 +377,12 @@ __device__ __forceinline__ void bw_store_rows(__nv_bfloat16* dst, int64_t ld, in
                  : "memory");
     if (r < rows) *reinterpret_cast<uint4*>(dst + r * ld + (lane & 7) * 8) = u;
   }
-  __syncwarp();
 }
 
 // KEYS: the key pass (rows are keys, columns are queries), else the query pass.  `first` is this
 // CTA's first item.  Returns false if a bounded wait gave up.
-template <bool KEYS>
+enum { BW_FEED, BW_COMPUTE, BW_STORE };
+template <bool KEYS, int ROLE>
 __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtensorMap& tm_qkv_cols,
                                         const CUtensorMap& tm_dout, const CUtensorMap& tm_dout_cols,
                                         const BwArgs& a, int first, uint32_t base, uint32_t bar_base,
@@ -312,13 +398,13 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
   BwItem it;
   it.start(a, first);
 
-  if (warp == BW_PRODUCER) {
+  if (ROLE == BW_FEED && warp == BW_PRODUCER) {
     // ---------------------------------------------------------------- producer
     uint32_t c = 0, lap = 0, loads = 0, ord = 0;
     for (; it.valid(a) && ok; it.next(a), ++ord) {
       const uint32_t ab = ord & 1;
       const int col = it.head * 64, row0 = it.tile * BW_TILE;
-      if (!mbar_wait(bar(WB_A_EMPTY + ab), ((ord >> 1) & 1) ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
+      if (!bw_wait(bar(WB_A_EMPTY + ab), ((ord >> 1) & 1) ^ 1u)) { ok = false; break; }
       if (lane == 0) {
         const uint32_t dst = sA + ab * 2 * BW_A_BYTES;
         mbar_expect_tx(bar(WB_A_FULL + ab), 2 * BW_A_BYTES);
@@ -329,8 +415,9 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
       __syncwarp();
       const float* lse_head = a.neg_lse2 + int64_t(it.head) * a.T;
       const float* delta_head = a.neg_delta + int64_t(it.head) * a.T;
+#pragma unroll 1
       for (int j = 0; j < it.n; ++j) {
-        if (!mbar_wait(bar(WB_EMPTY + c), (lap & 1) ^ 1u, status, ST_ATTN_TIMEOUT)) { ok = false; break; }
+        if (!bw_wait(bar(WB_DONE + c), lap ^ 1u)) { ok = false; break; }
         const int col0 = it.col0(j);
         if (KEYS) {
 #pragma unroll
@@ -340,154 +427,233 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
             cp_async4(dst, lse_head + q);
             cp_async4(dst + BW_COLS * 4, delta_head + q);
           }
-          cp_async_arrive(bar(WB_FULL + c));
+          cp_async_arrive(bar(WB_IN + c));
         }
         if (lane == 0) {
           const uint32_t dst = sB + c * 2 * BW_B_BYTES;
-          mbar_expect_tx(bar(WB_FULL + c), 2 * BW_B_BYTES);
-          tma_load_2d(dst, &tm_qkv_cols, bar(WB_FULL + c), (KEYS ? 0 : H) + col, col0);
-          if (KEYS) tma_load_2d(dst + BW_B_BYTES, &tm_dout_cols, bar(WB_FULL + c), col, col0);
-          else tma_load_2d(dst + BW_B_BYTES, &tm_qkv_cols, bar(WB_FULL + c), 2 * H + col, col0);
+          mbar_expect_tx(bar(WB_IN + c), 2 * BW_B_BYTES);
+          tma_load_2d(dst, &tm_qkv_cols, bar(WB_IN + c), (KEYS ? 0 : H) + col, col0);
+          if (KEYS) tma_load_2d(dst + BW_B_BYTES, &tm_dout_cols, bar(WB_IN + c), col, col0);
+          else tma_load_2d(dst + BW_B_BYTES, &tm_qkv_cols, bar(WB_IN + c), 2 * H + col, col0);
         }
         __syncwarp();
         ++loads;
-        if (++c == BW_SLOTS) {
-          c = 0;
-          ++lap;
-        }
+        c = bw_next_slot(c);
+        lap ^= c == 0;
       }
     }
-    if (!ok) {  // gave up: this CTA's copies must have landed before it can leave
-      for (uint32_t u = loads > BW_SLOTS ? loads - BW_SLOTS : 0; u < loads; ++u)
-        mbar_wait(bar(WB_FULL + u % BW_SLOTS), (u / BW_SLOTS) & 1, status, ST_ATTN_TIMEOUT);
-      for (uint32_t u = ord > 1 ? ord - 2 : 0; u <= ord; ++u)  // (one that was never issued runs into its limit)
-        mbar_wait(bar(WB_A_FULL + (u & 1)), (u >> 1) & 1, status, ST_ATTN_TIMEOUT);
+    // three tiles that are not there arrive empty, so that every tile's dS finds its barrier
+#pragma unroll 1
+    for (int j = 0; j < BW_GROUPS && ok && loads > 0; ++j) {
+      if (!bw_wait(bar(WB_DONE + c), lap ^ 1u)) { ok = false; break; }
+      if (KEYS) mbar_arrive(bar(WB_IN + c));
+      if (lane == 0) mbar_arrive(bar(WB_IN + c));
+      c = bw_next_slot(c);
+        lap ^= c == 0;
     }
-  } else if (warp == BW_MMA) {
+    if (!ok) {  // gave up: this CTA's copies must have landed before it can leave
+      set_status(status, ST_ATTN_TIMEOUT);
+#pragma unroll 1
+      for (uint32_t u = loads > BW_SLOTS ? loads - BW_SLOTS : 0; u < loads; ++u)
+        bw_wait(bar(WB_IN + u % BW_GROUPS * 2 + u / BW_GROUPS % 2), (u / BW_SLOTS) & 1);
+#pragma unroll 1
+      for (uint32_t u = ord > 1 ? ord - 2 : 0; u <= ord; ++u)  // (one that was never issued runs into its limit)
+        bw_wait(bar(WB_A_FULL + (u & 1)), (u >> 1) & 1);
+    }
+  } else if (ROLE == BW_FEED && warp == BW_MMA) {
     // ---------------------------------------------------------------- MMA issuer
     // The scores run three tiles ahead of the accumulation and dP two, so that by the time something
-    // is waited for it has usually happened: this one thread feeds the tensor core with four
-    // products per tile and its own latency counts.
+    // is waited for it has usually happened.  This one thread is what bounds the kernel: an MMA costs it
+    // 23 clocks to issue on an idle scheduler and 32 beside busy warps (sixteen per tile), a look at a
+    // barrier about a hundred.  So a tile needs two barriers only (WB_IN stands for two events, and
+    // P and dS are announced together), and their state is asked for ahead of four MMAs and read after
+    // them.  Electing a lane for each group of MMAs inside a loop of the whole warp, which would keep the
+    // descriptors in uniform registers, made it 100 clocks per MMA.
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc_bf16(BW_TILE, BW_COLS, 0);
       constexpr uint32_t idesc_acc = umma_idesc_bf16(BW_TILE, 64, 1);  // B is MN-major: its rows are the contraction
-      auto wait = [&](int b, uint32_t parity) {
-        if (ok && !mbar_wait(bar(b), parity, status, ST_ATTN_MMA_TIMEOUT)) ok = false;
-        return ok;
-      };
-      auto buffer = [&](uint32_t c) { return tmem_base + (c >= BW_GROUPS ? (c - BW_GROUPS) * 128 + 64 : c * 128); };
       const uint64_t a_desc = umma_smem_desc_sw128(sA, 1024), b_desc = umma_smem_desc_sw128(sB, 1024);
-      auto scores = [&](uint32_t d, uint64_t ad, uint64_t bd) {
+      const uint32_t desc_hi = uint32_t(a_desc >> 32);  // the same for both
+      auto desc = [&](uint32_t lo) { return (uint64_t(desc_hi) << 32) | lo; };
+      auto scores = [&](uint32_t d, uint32_t ad, uint32_t bd) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) umma_ss(d, ad + 2u * kk, bd + 2u * kk, idesc_s, kk != 0 ? 1u : 0u);
+        for (int kk = 0; kk < 4; ++kk) umma_ss(d, desc(ad + 2u * kk), desc(bd + 2u * kk), idesc_s, kk != 0 ? 1u : 0u);
       };
       // acc += X B, X (bf16 pairs of 64 columns) in tensor memory
-      auto accumulate = [&](uint32_t acc_col, uint32_t x, uint64_t bd, bool first_tile) {
+      auto accumulate = [&](uint32_t acc_col, uint32_t x, uint32_t bd, uint32_t add) {
 #pragma unroll
         for (int kk = 0; kk < BW_COLS / 16; ++kk)
-          g_umma_ts(tmem_base + acc_col, x + kk * 8, bd + uint32_t(kk * 2048 >> 4), idesc_acc,
-                    (!first_tile || kk != 0) ? 1u : 0u);
+          g_umma_ts(tmem_base + acc_col, x + kk * 8, desc(bd + uint32_t(kk * 2048 >> 4)), idesc_acc, kk != 0 ? 1u : add);
       };
       // A tile on its way from scores to accumulation: A buffer (1), first (2) and last (4) of its
       // item, present (8)
-      int j = 0;
-      uint32_t ord = 0, a_loads = 0;
+      int left = it.valid(a) ? it.n : 0;  // tiles of the item whose scores come next
+      uint32_t fresh = 2u, ab = 0, a_phase = 0;
       auto next_tile = [&]() {
-        if (!it.valid(a)) return 0u;
-        const uint32_t f = 8u | (ord & 1) | (j == 0 ? 2u : 0u) | (j + 1 == it.n ? 4u : 0u);
-        if (++j == it.n) {
-          j = 0;
-          ++ord;
+        if (left == 0) return 0u;
+        uint32_t f = 8u | ab | fresh;
+        fresh = 0;
+        if (--left == 0) {
+          f |= 4u;
+          fresh = 2u;
+          ab ^= 1u;
           it.next(a);
+          left = it.valid(a) ? it.n : 0;
         }
         return f;
       };
-      auto issue_s = [&](uint32_t f, uint32_t c, uint32_t lap) {  // of the tile in slot c
+      const uint32_t a_lo = uint32_t(a_desc), b_lo = uint32_t(b_desc);
+      auto issue_s = [&](uint32_t f, uint32_t c) {  // of the tile in slot c, whose columns have arrived
         if (f & 2u) {
-          if (!wait(WB_A_FULL + (f & 1), (a_loads >> 1) & 1)) return;
-          ++a_loads;
+          if (!bw_wait(bar(WB_A_FULL) + (f & 1) * 8u, a_phase >> 1)) return false;
+          a_phase = (a_phase + 1) & 3u;
+          tc_fence_after();
         }
-        if (!wait(WB_FULL + c, lap & 1)) return;
+        scores(tmem_base + c * 64, a_lo + (f & 1) * (2 * BW_A_BYTES >> 4), b_lo + c * (2 * BW_B_BYTES >> 4));
+        umma_commit(bar(WB_S_FULL) + c * 8u);
+        return true;
+      };
+      auto issue_dp = [&](uint32_t f, uint32_t c) {
+        scores(tmem_base + (c ^ 1u) * 64, a_lo + ((f & 1) * 2 + 1) * (BW_A_BYTES >> 4),
+               b_lo + (c * 2 + 1) * (BW_B_BYTES >> 4));
+        umma_commit(bar(WB_DP_FULL) + c * 8u);
+        if (f & 4u) umma_commit(bar(WB_A_EMPTY) + (f & 1) * 8u);
+      };
+      uint32_t f0 = 0, f1 = 0, f2 = 0;  // tiles g, g + 1, g + 2
+#pragma unroll 1
+      for (uint32_t g = 0; g < BW_GROUPS && ok; ++g) {
+        f0 = f1;
+        f1 = f2;
+        f2 = next_tile();
+        if (!f2) continue;
+        ok = bw_wait(bar(WB_IN) + g * 16u, 0);
         tc_fence_after();
-        scores(buffer(c), a_desc + (f & 1) * (2 * BW_A_BYTES >> 4), b_desc + c * (2 * BW_B_BYTES >> 4));
-        umma_commit(bar(WB_S_FULL + c));
-      };
-      auto issue_dp = [&](uint32_t f, uint32_t c) {  // its operands arrived with those of its scores
-        scores(buffer(c) ^ 64u, a_desc + ((f & 1) * 2 + 1) * (BW_A_BYTES >> 4),
-               b_desc + (c * 2 + 1) * (BW_B_BYTES >> 4));
-        umma_commit(bar(WB_DP_FULL + c));
-        if (f & 4u) umma_commit(bar(WB_A_EMPTY + (f & 1)));
-      };
-      uint32_t f0 = next_tile(), f1 = next_tile(), f2 = next_tile();  // tiles g, g + 1, g + 2
-      if (f0) {
-        issue_s(f0, 0, 0);
-        if (ok) issue_dp(f0, 0);
+        ok = ok && issue_s(f2, g * 2);
+        if (ok && g < 2) issue_dp(f2, g * 2);
       }
-      if (f1 && ok) {
-        issue_s(f1, 1, 0);
-        if (ok) issue_dp(f1, 1);
-      }
-      if (f2 && ok) issue_s(f2, 2, 0);
-      uint32_t c = 0, lap = 0, items = 0;  // slot and lap of tile g, items whose accumulation has begun
+      // Slots of tiles g and g - 1 and the parities of their laps (before the first tile: of a barrier's
+      // state before its first phase).
+      uint32_t c = 0, lap = 0, cm = BW_SLOTS - 1, lapm = 1;
+      uint32_t acc_phase = KEYS ? 1u : 2u, acc_col = tmem_base + BW_ACC1_COL, acc_bar = 0;
+      uint32_t f3 = next_tile();  // tile g + 3
+      bool in = false;
+#pragma unroll 1
       while (ok && f0) {
-        const uint64_t b1 = b_desc + c * (2 * BW_B_BYTES >> 4);
-        const bool fresh = (f0 & 2u) != 0;
-        if (fresh) {  // the previous item's accumulators must have been read before they are overwritten
-          if (items > 0 && !wait(WB_ACC_EMPTY, (items - 1) & 1)) break;
-          ++items;
-        }
-        if (KEYS) {
-          if (!wait(WB_P_FULL + c, lap & 1)) break;
-          tc_fence_after();
-          accumulate(BW_ACC2_COL, buffer(c), b1 + (BW_B_BYTES >> 4), fresh);  // dV += P^T dO
-        }
-        const uint32_t f3 = next_tile();
-        if (f3) {  // dP of tile g has been read: its buffer takes the scores of tile g + 3
-          const uint32_t c3 = c >= BW_GROUPS ? c - BW_GROUPS : c + BW_GROUPS;
-          if (!wait(WB_DP_READ + c, lap & 1)) break;
-          issue_s(f3, c3, lap + (c >= BW_GROUPS ? 1 : 0));
-          if (!ok) break;
-        }
-        if (f2) {  // P and dS of tile g - 1 have been multiplied: their buffer takes dP of tile g + 2
-          const uint32_t cm = c == 0 ? BW_SLOTS - 1 : c - 1;
-          if ((c | lap) != 0 && !wait(WB_DK_DONE + cm, (lap - (c == 0 ? 1 : 0)) & 1)) break;
-          tc_fence_after();
-          issue_dp(f2, c + 2 >= BW_SLOTS ? c + 2 - BW_SLOTS : c + 2);
-        }
-        if (!wait(WB_DS_FULL + c, lap & 1)) break;
+        // dS of tile g is written (its dP has been read) and the columns of tile g + 3 are here
+        if (!in && !bw_wait(bar(WB_IN) + (c ^ 1u) * 8u, (lap ^ c) & 1u)) { ok = false; break; }
         tc_fence_after();
-        accumulate(BW_ACC1_COL, buffer(c) + 32, b1, fresh);  // dK += dS^T Q, dQ += dS K
-        umma_commit(bar(WB_DK_DONE + c));
-        umma_commit(bar(WB_EMPTY + c));
+        bool done;
+        if (f3) {
+          if (f3 & 2u) {
+            if (!bw_wait(bar(WB_A_FULL) + (f3 & 1) * 8u, a_phase >> 1)) { ok = false; break; }
+            a_phase = (a_phase + 1) & 3u;
+            tc_fence_after();
+          }
+          done = bw_products_ss(tmem_base + (c ^ 1u) * 64, a_lo + (f3 & 1) * (2 * BW_A_BYTES >> 4),
+                                b_lo + (c ^ 1u) * (2 * BW_B_BYTES >> 4), desc_hi, idesc_s,
+                                bar(WB_S_FULL) + (c ^ 1u) * 8u, bar(WB_DONE) + cm * 8u, lapm);
+        } else {
+          done = false;
+        }
+        const uint32_t x = tmem_base + c * 64, b1 = b_lo + c * (2 * BW_B_BYTES >> 4);
+        uint32_t add = 1;
+        if (f0 & 2u) {  // the previous item's accumulators must have been read before they are overwritten
+          if (KEYS) {
+            if (!bw_wait(bar(WB_ACC_EMPTY), acc_phase)) { ok = false; break; }
+            acc_phase ^= 1u;
+          } else {  // dQ needs one accumulator only: items take the two in turn
+            acc_bar = (f0 & 1) * 8u;
+            if (!bw_wait(bar(WB_ACC_EMPTY) + acc_bar, acc_phase >> 1)) { ok = false; break; }
+            acc_phase = (acc_phase + 1) & 3u;
+            acc_col = tmem_base + BW_ACC1_COL + (f0 & 1) * 64;
+          }
+          tc_fence_after();
+          add = 0;
+        }
+        if (KEYS) accumulate(BW_ACC2_COL, x, b1 + (BW_B_BYTES >> 4), add);  // dV += P^T dO
+        const uint32_t f4 = next_tile();
+        if (f2) {  // P and dS of tile g - 1 have been multiplied: their buffer takes dP of tile g + 2
+          if (!done && !bw_wait(bar(WB_DONE) + cm * 8u, lapm)) { ok = false; break; }
+          tc_fence_after();
+          issue_dp(f2, cm ^ 1u);
+        }
+        const uint32_t c_next = bw_next_slot(c), lap_next = lap ^ (c_next == 0 ? 1u : 0u);
+        // dK += dS^T Q, dQ += dS K
+        in = bw_products_ts(acc_col, x + 32, b1, desc_hi, idesc_acc, add, bar(WB_DONE) + c * 8u,
+                            bar(WB_IN) + (c_next ^ 1u) * 8u, (lap_next ^ c_next) & 1u);
+        if (f0 & 4u) umma_commit(bar(WB_ACC_FULL) + acc_bar);
         f0 = f1;
         f1 = f2;
         f2 = f3;
-        if (++c == BW_SLOTS) {
-          c = 0;
-          ++lap;
-        }
+        f3 = f4;
+        cm = c;
+        lapm = lap;
+        c = c_next;
+        lap = lap_next;
       }
+      if (!ok) set_status(status, ST_ATTN_MMA_TIMEOUT);
     }
     __syncwarp();
     ok = __all_sync(0xffffffffu, ok);
-  } else {
+  } else if (ROLE == BW_STORE) {
+    // ---------------------------------------------------------------- gradients out of the accumulators
+    const int row = (warp & 3) * 32 + lane;  // row of the tile = tensor-memory lane
+    const uint32_t lane_addr = tmem_base + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t block = base + BW_OUT_OFFSET + (warp & 3) * BW_OUT_BYTES;
+    uint32_t ord = 0;
+#pragma unroll 1
+    for (; it.valid(a); it.next(a), ++ord) {
+      const int t = it.tile * BW_TILE + row;
+      bool empty = true;
+      const uint4* trow = nullptr;
+      if (t < a.T) {
+        const int2 range = __ldg(a.row_range + t);
+        empty = range.x >= range.y;  // rows that attend nothing are exact zeros
+        if (a.pos != nullptr) {
+          int64_t ps = a.pos[t];
+          if (ps < 0 || ps >= a.max_positions) {
+            set_status(status, ST_BAD_POSITION);
+            ps = 0;
+          }
+          trow = reinterpret_cast<const uint4*>(a.table + ps * 64);
+        }
+      }
+      const uint32_t b = KEYS ? 0 : ord & 1, phase = KEYS ? ord & 1 : (ord >> 1) & 1;
+      if (ok) ok = bw_wait(bar(WB_ACC_FULL) + b * 8, phase);
+      tc_fence_after();
+      bw_finish_row(lane_addr + BW_ACC1_COL + b * 64, 0.125f, trow, empty, block, lane);
+      if (KEYS) bw_finish_row(lane_addr + BW_ACC2_COL, 1.0f, nullptr, empty, block + 32 * 128, lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(WB_ACC_EMPTY) + b * 8);
+      const int row0 = it.tile * BW_TILE + (warp & 3) * 32;
+      const int rows = ok ? a.T - row0 : 0;
+      const int64_t ld = 3 * int64_t(H);
+      __nv_bfloat16* dst = a.dqkv + row0 * ld + (KEYS ? H : 0) + it.head * 64;
+      bw_store_rows(dst, ld, rows, block, lane);
+      if (KEYS) bw_store_rows(dst + H, ld, rows, block + 32 * 128, lane);
+      __syncwarp();
+    }
+    if (!ok) set_status(status, ST_ATTN_SOFTMAX_TIMEOUT);
+  } else if (ROLE == BW_COMPUTE) {
     // ---------------------------------------------------------------- compute warps
     const int w = warp >> 2;                         // group
     const int row = (warp & 3) * 32 + lane;          // row of the tile = tensor-memory lane
     const uint32_t lane_addr = tmem_base + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t out_block = base + BW_OUT_OFFSET + warp * BW_OUT_BYTES;
     const float scale_log2 = 0.125f * 1.4426950408889634f;  // 1/sqrt(64) * log2(e)
     const float2 scale2 = make_float2(scale_log2, scale_log2);
     // After a bounded wait has given up the loops still run to their end, without waiting, so that
     // every thread reaches the common exit.
     auto wait = [&](int b, uint32_t parity) {
-      if (ok && !mbar_wait(bar(b), parity, status, ST_ATTN_SOFTMAX_TIMEOUT)) ok = false;
+      if (ok) ok = bw_wait(bar(b), parity);
     };
+    auto test = [&](int b, uint32_t parity) { return bw_test(bar(b), parity); };
     auto arrive = [&](int b) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(b));
     };
+    if (lane == 0) mbar_arrive(bar(WB_IN + 2 * w));  // no tile comes three before the first three
     int j = w;       // this group's next tile, counted from the item's first
     uint32_t i = 0;  // tiles of this group so far
     for (; it.valid(a); it.next(a)) {
@@ -505,21 +671,32 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
           }
         }
         for (; j < it.n; j += BW_GROUPS, ++i) {
-          const uint32_t c = w + (i & 1) * BW_GROUPS, lap = (i >> 1) & 1;
-          const uint32_t s_addr = lane_addr + w * 128 + (i & 1) * 64;
+          const uint32_t c = 2 * w + (i & 1), lap = (i >> 1) & 1;
+          const uint32_t s_addr = lane_addr + c * 64;
           const uint32_t dp_addr = s_addr ^ 64u;
           const uint32_t stats = sStats + c * BW_STATS_BYTES;
+          const bool s_full = test(WB_S_FULL + c, lap), b_full = !KEYS || test(WB_IN + c, lap);
           // valid columns of this row within the tile: [c_lo, c_hi)
           const int x0 = it.col0(j);
           const int c_lo = max(range.x, it.lo + j * BW_COLS) - x0, c_hi = range.y - x0;
           const bool full = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= BW_COLS);
-          wait(WB_S_FULL + c, lap);
-          if (KEYS) wait(WB_FULL + c, lap);  // complete by now: makes lse and delta visible
+          const bool none = __all_sync(0xffffffffu, c_lo >= c_hi || c_hi <= 0 || c_lo >= BW_COLS);
+          if (!s_full) wait(WB_S_FULL + c, lap);
+          if (!b_full) wait(WB_IN + c, lap);  // complete by now: makes lse and delta visible
           tc_fence_after();
+          if (none) {
+            uint32_t zero[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) zero[e] = 0;
+            wait(WB_DP_FULL + c, lap);
+#pragma unroll 1
+            for (int h = KEYS ? 0 : 2; h < 4; ++h) g_tmem_st16(s_addr + h * 16, zero);
+          } else {
           uint32_t p[64];
           g_tmem_ld32(s_addr, p);
           tmem_ld_wait();
           g_tmem_ld32(s_addr + 32, p + 32);  // in flight during the first half's exponentials
+          const bool dp_full = test(WB_DP_FULL + c, lap);
           auto exponentials = [&](int e0) {
 #pragma unroll
             for (int e = e0; e < e0 + 32; e += 4) {
@@ -540,8 +717,13 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
           tmem_ld_wait();
           exponentials(32);
           if (!full) {
+            // columns [c_lo, c_hi) of the tile as bits
+            const uint32_t m0 = bw_bits(c_lo, c_hi), m1 = bw_bits(c_lo - 32, c_hi - 32);
 #pragma unroll
-            for (int e = 0; e < BW_COLS; ++e) p[e] = (e >= c_lo && e < c_hi) ? p[e] : 0u;
+            for (int e = 0; e < 32; ++e) {
+              p[e] = (m0 >> e & 1u) ? p[e] : 0u;
+              p[e + 32] = (m1 >> e & 1u) ? p[e + 32] : 0u;
+            }
           }
           if (KEYS) {  // P^T in place of the first half of the scores: the A operand of dV += P^T dO
 #pragma unroll
@@ -552,10 +734,8 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
                 pk[e] = pack_bf16(__uint_as_float(p[h * 32 + 2 * e]), __uint_as_float(p[h * 32 + 2 * e + 1]));
               g_tmem_st16(s_addr + h * 16, pk);
             }
-            g_tmem_st_wait();
-            arrive(WB_P_FULL + c);
           }
-          wait(WB_DP_FULL + c, lap);
+          if (!dp_full) wait(WB_DP_FULL + c, lap);
           tc_fence_after();
           uint32_t dp[2][16];
           g_tmem_ld16(dp_addr, dp[0]);
@@ -563,7 +743,6 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
           for (int h = 0; h < 4; ++h) {
             tmem_ld_wait();
             if (h < 3) g_tmem_ld16(dp_addr + (h + 1) * 16, dp[(h + 1) & 1]);  // in flight during this quarter
-            else arrive(WB_DP_READ + c);
             const uint32_t* d = dp[h & 1];
             uint32_t pk[8];
 #pragma unroll
@@ -583,41 +762,39 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
             }
             g_tmem_st8(s_addr + 32 + h * 8, pk);  // dS in place of the second half
           }
-          g_tmem_st_wait();
-          arrive(WB_DS_FULL + c);
-          if (j + 1 == it.n) {
-            // The group of an item's last tile stores its gradients while the others go on; the row's 64
-            // (or twice 64) values are in registers before the accumulators are handed back.  Rows
-            // that attend nothing are exact zeros.
-            const uint4* trow = nullptr;
-            if (a.pos != nullptr && t < a.T) {
-              int64_t ps = a.pos[t];
-              if (ps < 0 || ps >= a.max_positions) {
-                set_status(status, ST_BAD_POSITION);
-                ps = 0;
-              }
-              trow = reinterpret_cast<const uint4*>(a.table + ps * 64);
-            }
-            wait(WB_DK_DONE + c, lap);
-            tc_fence_after();
-            uint32_t v1[32], v2[32];
-            bw_finish_row(lane_addr + BW_ACC1_COL, 0.125f, trow, v1);
-            if (KEYS) bw_finish_row(lane_addr + BW_ACC2_COL, 1.0f, nullptr, v2);
-            arrive(WB_ACC_EMPTY);
-            const bool empty = range.x >= range.y;
-            const int row0 = it.tile * BW_TILE + (warp & 3) * 32;
-            const int rows = ok ? a.T - row0 : 0;
-            const int64_t ld = 3 * int64_t(H);
-            __nv_bfloat16* dst = a.dqkv + row0 * ld + (KEYS ? H : 0) + it.head * 64;
-            bw_store_rows(dst, ld, rows, out_block, lane, v1, empty);
-            if (KEYS) bw_store_rows(dst + H, ld, rows, out_block, lane, v2, empty);
           }
+          g_tmem_st_wait();
+          arrive(WB_IN + (c ^ 1u));
         }
       }
       j -= it.n;
     }
+    if (!ok) set_status(status, ST_ATTN_SOFTMAX_TIMEOUT);
   }
   return ok;
+}
+
+template <int ROLE>
+__device__ __forceinline__ void bw_both(const CUtensorMap& tm_qkv, const CUtensorMap& tm_qkv_cols,
+                                        const CUtensorMap& tm_dout, const CUtensorMap& tm_dout_cols,
+                                        const BwArgs& a, int second, uint32_t base, uint32_t bar_base,
+                                        uint32_t tmem_base) {
+  const bool ok = bw_pass<true, ROLE>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, blockIdx.x, base, bar_base,
+                                         tmem_base);
+  tc_fence_before();
+  uint32_t failed;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 0, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(failed)
+      : "r"(ok ? 0u : 1u)
+      : "memory");
+  tc_fence_after();
+  if (!failed)
+    bw_pass<false, ROLE>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, second, base, bar_base + WB_COUNT * 8,
+                            tmem_base);
 }
 
 __global__ void __launch_bounds__(BW_THREADS, 1)
@@ -638,9 +815,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
       const uint32_t bb = bar_base + pass * WB_COUNT * 8;
       for (int i = 0; i < WB_COUNT; ++i) {
         uint32_t count = 1;
-        // stages of the key pass: the TMA issue and 32 lanes' copies of lse and delta
-        if (pass == 0 && i >= WB_FULL && i < WB_FULL + BW_SLOTS) count = 33;
-        if (i >= WB_P_FULL) count = 4;
+        // four compute warps, the TMA issue and in the key pass 32 lanes' copies of lse and delta
+        if (i < WB_IN + BW_SLOTS) count = pass == 0 ? 37 : 5;
+        if (i >= WB_ACC_EMPTY) count = 4;
         mbar_init(bb + 8u * i, count);
       }
     }
@@ -662,14 +839,17 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
 
   // Items of both passes form one list, the key pass first; a CTA takes every gridDim-th of it, so
   // the passes need no launch boundary and a small batch runs both at the same time.
-  const bool ok = bw_pass<true>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, blockIdx.x, base, bar_base, tmem_base);
-  tc_fence_before();
-  const int failed = __syncthreads_or(!ok);
-  tc_fence_after();
-  if (!failed) {
-    int first = int(blockIdx.x) - a.n_items % int(gridDim.x);
-    if (first < 0) first += gridDim.x;
-    bw_pass<false>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, first, base, bar_base + WB_COUNT * 8, tmem_base);
+  int second = int(blockIdx.x) - a.n_items % int(gridDim.x);
+  if (second < 0) second += gridDim.x;
+  if (warp < BW_COMPUTE_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+    bw_both<BW_COMPUTE>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, second, base, bar_base, tmem_base);
+  } else if (warp < BW_STORER) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    bw_both<BW_FEED>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, second, base, bar_base, tmem_base);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    bw_both<BW_STORE>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, second, base, bar_base, tmem_base);
   }
   tc_fence_before();
   __syncthreads();
