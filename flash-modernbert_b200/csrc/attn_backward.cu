@@ -67,14 +67,14 @@ constexpr uint32_t BW_ACC2_COL = 448;  // dV; dQ of odd items
 
 // Barriers of one pass; each pass has its own set.  [c]: one per slot.
 enum {
-  WB_IN = 0,                            // [c] the tile's operands are here and dS of the tile three before it is written
+  WB_IN = 0,                            // [c] the tile's operands are here, dS of the tile three before it is written
   WB_S_FULL = WB_IN + BW_SLOTS,         // [c]
   WB_DP_FULL = WB_S_FULL + BW_SLOTS,    // [c]
   WB_DONE = WB_DP_FULL + BW_SLOTS,      // [c] the tile has been accumulated
   WB_A_FULL = WB_DONE + BW_SLOTS,       // [2]
   WB_A_EMPTY = WB_A_FULL + 2,           // [2]
-  WB_ACC_FULL = WB_A_EMPTY + 2,         // [2]
-  WB_ACC_EMPTY = WB_ACC_FULL + 2,       // [2] the item's accumulators have been read
+  WB_ACC_FULL = WB_A_EMPTY + 2,         // [2] one per accumulator
+  WB_ACC_EMPTY = WB_ACC_FULL + 2,       // [2] it has been read
   WB_COUNT = WB_ACC_EMPTY + 2
 };
 constexpr int BW_OUT_OFFSET = 4 * BW_A_BYTES + BW_SLOTS * 2 * BW_B_BYTES;
@@ -98,7 +98,8 @@ struct BwArgs {
 
 // ---- preparation ------------------------------------------------------------------
 // Grid (tiles, heads), 256 threads.  Every block: delta of its 128 rows and head, eight lanes per
-// row, and lse in the exponent's base, both negated as the passes use them.  Blocks of head 0 also find each row's sequence and window.
+// row, and lse in the exponent's base, both negated as the passes use them.  Blocks of head 0 also find
+// each row's sequence and window.
 // Boundaries are not trusted: a row whose sequence does not come out as begin <= t < end within
 // [0, T] attends nothing, and an entry outside [0, T] or below its predecessor is reported.
 __global__ void __launch_bounds__(256)
@@ -131,7 +132,7 @@ attn_bwd_prepare_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat
     }
   }
   if (head != 0) return;
-  for (int n = blockIdx.x * blockDim.x + threadIdx.x; n < n_seqs; n += gridDim.x * blockDim.x) {
+  for (int64_t n = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; n < n_seqs; n += int64_t(gridDim.x) * blockDim.x) {
     const int b = cu_seqlens[n], e = cu_seqlens[n + 1];
     if (b < 0 || e < b || e > T) set_status(status, ST_BAD_CU_SEQLENS);
   }
@@ -302,7 +303,9 @@ __device__ __forceinline__ bool bw_products_ts(uint32_t d, uint32_t a, uint32_t 
   return done != 0;
 }
 // Slot of the tile after the one in slot c: 0, 2, 4, 1, 3, 5, 0, ...
-__device__ __forceinline__ uint32_t bw_next_slot(uint32_t c) { return c + 2 < BW_SLOTS ? c + 2 : BW_SLOTS + 1 - (c + 2); }
+__device__ __forceinline__ uint32_t bw_next_slot(uint32_t c) {
+  return c + 2 < BW_SLOTS ? c + 2 : BW_SLOTS + 1 - (c + 2);
+}
 // Bits [lo, hi) of a word.
 __device__ __forceinline__ uint32_t bw_bits(int lo, int hi) {
   const uint32_t below_hi = hi >= 32 ? 0xffffffffu : (1u << max(hi, 0)) - 1u;
@@ -338,8 +341,8 @@ __device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, co
       float x[8], y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = empty ? 0.f : __uint_as_float(lo[h * 8 + e]) * scale;
-        y[e] = empty ? 0.f : __uint_as_float(hi[h * 8 + e]) * scale;
+        x[e] = __uint_as_float(lo[h * 8 + e]) * scale;
+        y[e] = __uint_as_float(hi[h * 8 + e]) * scale;
       }
       if (trow != nullptr) {
         float cs[8], sn[8];
@@ -363,6 +366,11 @@ __device__ __forceinline__ void bw_finish_row(uint32_t acc_addr, float scale, co
                    "r"(pack_bf16(y[6], y[7]))
                    : "memory");
     }
+  }
+  if (empty) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(block + lane * 128 + (i << 4)), "r"(0) : "memory");
   }
 }
 // The block's rows to memory, four whole rows per instruction; `dst` is the first row's, `rows` how many of them exist.
@@ -483,7 +491,8 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
       auto accumulate = [&](uint32_t acc_col, uint32_t x, uint32_t bd, uint32_t add) {
 #pragma unroll
         for (int kk = 0; kk < BW_COLS / 16; ++kk)
-          g_umma_ts(tmem_base + acc_col, x + kk * 8, desc(bd + uint32_t(kk * 2048 >> 4)), idesc_acc, kk != 0 ? 1u : add);
+          g_umma_ts(tmem_base + acc_col, x + kk * 8, desc(bd + uint32_t(kk * 2048 >> 4)), idesc_acc,
+                    kk != 0 ? 1u : add);
       };
       // A tile on its way from scores to accumulation: A buffer (1), first (2) and last (4) of its
       // item, present (8)
@@ -559,8 +568,7 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
         uint32_t add = 1;
         if (f0 & 2u) {  // the previous item's accumulators must have been read before they are overwritten
           if (KEYS) {
-            if (!bw_wait(bar(WB_ACC_EMPTY), acc_phase)) { ok = false; break; }
-            acc_phase ^= 1u;
+            if (!bw_wait(bar(WB_ACC_EMPTY + 1), acc_phase)) { ok = false; break; }
           } else {  // dQ needs one accumulator only: items take the two in turn
             acc_bar = (f0 & 1) * 8u;
             if (!bw_wait(bar(WB_ACC_EMPTY) + acc_bar, acc_phase >> 1)) { ok = false; break; }
@@ -570,12 +578,20 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
           tc_fence_after();
           add = 0;
         }
-        if (KEYS) accumulate(BW_ACC2_COL, x, b1 + (BW_B_BYTES >> 4), add);  // dV += P^T dO
+        if (KEYS) {
+          accumulate(BW_ACC2_COL, x, b1 + (BW_B_BYTES >> 4), add);  // dV += P^T dO
+          if (f0 & 4u) umma_commit(bar(WB_ACC_FULL + 1));
+        }
         const uint32_t f4 = next_tile();
         if (f2) {  // P and dS of tile g - 1 have been multiplied: their buffer takes dP of tile g + 2
           if (!done && !bw_wait(bar(WB_DONE) + cm * 8u, lapm)) { ok = false; break; }
           tc_fence_after();
           issue_dp(f2, cm ^ 1u);
+        }
+        if (KEYS && !add) {
+          if (!bw_wait(bar(WB_ACC_EMPTY), acc_phase)) { ok = false; break; }
+          tc_fence_after();
+          acc_phase ^= 1u;
         }
         const uint32_t c_next = bw_next_slot(c), lap_next = lap ^ (c_next == 0 ? 1u : 0u);
         // dK += dS^T Q, dQ += dS K
@@ -618,14 +634,17 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
           trow = reinterpret_cast<const uint4*>(a.table + ps * 64);
         }
       }
-      const uint32_t b = KEYS ? 0 : ord & 1, phase = KEYS ? ord & 1 : (ord >> 1) & 1;
-      if (ok) ok = bw_wait(bar(WB_ACC_FULL) + b * 8, phase);
-      tc_fence_after();
-      bw_finish_row(lane_addr + BW_ACC1_COL + b * 64, 0.125f, trow, empty, block, lane);
-      if (KEYS) bw_finish_row(lane_addr + BW_ACC2_COL, 1.0f, nullptr, empty, block + 32 * 128, lane);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(WB_ACC_EMPTY) + b * 8);
+      auto take = [&](uint32_t b, uint32_t phase, float scale, const uint4* turn, uint32_t to) {
+        if (ok) ok = bw_wait(bar(WB_ACC_FULL) + b * 8, phase);
+        tc_fence_after();
+        bw_finish_row(lane_addr + BW_ACC1_COL + b * 64, scale, turn, empty, to, lane);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(WB_ACC_EMPTY) + b * 8);
+      };
+      if (KEYS) take(1, ord & 1, 1.0f, nullptr, block + 32 * 128);  // dV is complete before dK
+      if (KEYS) take(0, ord & 1, 0.125f, trow, block);
+      else take(ord & 1, (ord >> 1) & 1, 0.125f, trow, block);
       const int row0 = it.tile * BW_TILE + (warp & 3) * 32;
       const int rows = ok ? a.T - row0 : 0;
       const int64_t ld = 3 * int64_t(H);
@@ -684,7 +703,7 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
           if (!s_full) wait(WB_S_FULL + c, lap);
           if (!b_full) wait(WB_IN + c, lap);  // complete by now: makes lse and delta visible
           tc_fence_after();
-          if (none) {
+          if (none) {  // no row of this warp attends any of the columns
             uint32_t zero[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) zero[e] = 0;
@@ -692,76 +711,76 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
 #pragma unroll 1
             for (int h = KEYS ? 0 : 2; h < 4; ++h) g_tmem_st16(s_addr + h * 16, zero);
           } else {
-          uint32_t p[64];
-          g_tmem_ld32(s_addr, p);
-          tmem_ld_wait();
-          g_tmem_ld32(s_addr + 32, p + 32);  // in flight during the first half's exponentials
-          const bool dp_full = test(WB_DP_FULL + c, lap);
-          auto exponentials = [&](int e0) {
-#pragma unroll
-            for (int e = e0; e < e0 + 32; e += 4) {
-              float4 l;
-              if (KEYS) l = lds128(stats + e * 4);
-              else l = make_float4(neg_lse, neg_lse, neg_lse, neg_lse);
-              const float2 u = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), scale2,
-                                          make_float2(l.x, l.y));
-              const float2 v = __ffma2_rn(make_float2(__uint_as_float(p[e + 2]), __uint_as_float(p[e + 3])), scale2,
-                                          make_float2(l.z, l.w));
-              p[e] = __float_as_uint(g_ex2(u.x));
-              p[e + 1] = __float_as_uint(g_ex2(u.y));
-              p[e + 2] = __float_as_uint(g_ex2(v.x));
-              p[e + 3] = __float_as_uint(g_ex2(v.y));
-            }
-          };
-          exponentials(0);
-          tmem_ld_wait();
-          exponentials(32);
-          if (!full) {
-            // columns [c_lo, c_hi) of the tile as bits
-            const uint32_t m0 = bw_bits(c_lo, c_hi), m1 = bw_bits(c_lo - 32, c_hi - 32);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              p[e] = (m0 >> e & 1u) ? p[e] : 0u;
-              p[e + 32] = (m1 >> e & 1u) ? p[e + 32] : 0u;
-            }
-          }
-          if (KEYS) {  // P^T in place of the first half of the scores: the A operand of dV += P^T dO
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                pk[e] = pack_bf16(__uint_as_float(p[h * 32 + 2 * e]), __uint_as_float(p[h * 32 + 2 * e + 1]));
-              g_tmem_st16(s_addr + h * 16, pk);
-            }
-          }
-          if (!dp_full) wait(WB_DP_FULL + c, lap);
-          tc_fence_after();
-          uint32_t dp[2][16];
-          g_tmem_ld16(dp_addr, dp[0]);
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
+            uint32_t p[64];
+            g_tmem_ld32(s_addr, p);
             tmem_ld_wait();
-            if (h < 3) g_tmem_ld16(dp_addr + (h + 1) * 16, dp[(h + 1) & 1]);  // in flight during this quarter
-            const uint32_t* d = dp[h & 1];
-            uint32_t pk[8];
+            g_tmem_ld32(s_addr + 32, p + 32);  // in flight during the first half's exponentials
+            const bool dp_full = test(WB_DP_FULL + c, lap);
+            auto exponentials = [&](int e0) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              float4 dl;
-              if (KEYS) dl = lds128(stats + BW_COLS * 4 + (h * 16 + e) * 4);
-              else dl = make_float4(neg_delta, neg_delta, neg_delta, neg_delta);
-              const uint32_t* q = p + h * 16 + e;
-              const float2 u = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])),
-                                                     make_float2(dl.x, dl.y)),
-                                          make_float2(__uint_as_float(q[0]), __uint_as_float(q[1])));
-              const float2 v = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])),
-                                                     make_float2(dl.z, dl.w)),
-                                          make_float2(__uint_as_float(q[2]), __uint_as_float(q[3])));
-              pk[e / 2] = pack_bf16(u.x, u.y);
-              pk[e / 2 + 1] = pack_bf16(v.x, v.y);
+              for (int e = e0; e < e0 + 32; e += 4) {
+                float4 l;
+                if (KEYS) l = lds128(stats + e * 4);
+                else l = make_float4(neg_lse, neg_lse, neg_lse, neg_lse);
+                const float2 u = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), scale2,
+                                            make_float2(l.x, l.y));
+                const float2 v = __ffma2_rn(make_float2(__uint_as_float(p[e + 2]), __uint_as_float(p[e + 3])), scale2,
+                                            make_float2(l.z, l.w));
+                p[e] = __float_as_uint(g_ex2(u.x));
+                p[e + 1] = __float_as_uint(g_ex2(u.y));
+                p[e + 2] = __float_as_uint(g_ex2(v.x));
+                p[e + 3] = __float_as_uint(g_ex2(v.y));
+              }
+            };
+            exponentials(0);
+            tmem_ld_wait();
+            exponentials(32);
+            if (!full) {
+              // columns [c_lo, c_hi) of the tile as bits
+              const uint32_t m0 = bw_bits(c_lo, c_hi), m1 = bw_bits(c_lo - 32, c_hi - 32);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                p[e] = (m0 >> e & 1u) ? p[e] : 0u;
+                p[e + 32] = (m1 >> e & 1u) ? p[e + 32] : 0u;
+              }
             }
-            g_tmem_st8(s_addr + 32 + h * 8, pk);  // dS in place of the second half
-          }
+            if (KEYS) {  // P^T in place of the first half of the scores: the A operand of dV += P^T dO
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  pk[e] = pack_bf16(__uint_as_float(p[h * 32 + 2 * e]), __uint_as_float(p[h * 32 + 2 * e + 1]));
+                g_tmem_st16(s_addr + h * 16, pk);
+              }
+            }
+            if (!dp_full) wait(WB_DP_FULL + c, lap);
+            tc_fence_after();
+            uint32_t dp[2][16];
+            g_tmem_ld16(dp_addr, dp[0]);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              tmem_ld_wait();
+              if (h < 3) g_tmem_ld16(dp_addr + (h + 1) * 16, dp[(h + 1) & 1]);  // in flight during this quarter
+              const uint32_t* d = dp[h & 1];
+              uint32_t pk[8];
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                float4 dl;
+                if (KEYS) dl = lds128(stats + BW_COLS * 4 + (h * 16 + e) * 4);
+                else dl = make_float4(neg_delta, neg_delta, neg_delta, neg_delta);
+                const uint32_t* q = p + h * 16 + e;
+                const float2 u = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])),
+                                                       make_float2(dl.x, dl.y)),
+                                            make_float2(__uint_as_float(q[0]), __uint_as_float(q[1])));
+                const float2 v = __fmul2_rn(__fadd2_rn(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])),
+                                                       make_float2(dl.z, dl.w)),
+                                            make_float2(__uint_as_float(q[2]), __uint_as_float(q[3])));
+                pk[e / 2] = pack_bf16(u.x, u.y);
+                pk[e / 2 + 1] = pack_bf16(v.x, v.y);
+              }
+              g_tmem_st8(s_addr + 32 + h * 8, pk);  // dS in place of the second half
+            }
           }
           g_tmem_st_wait();
           arrive(WB_IN + (c ^ 1u));
