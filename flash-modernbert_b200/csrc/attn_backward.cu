@@ -27,6 +27,7 @@
 // one before, whose columns are masked out there), so rows behind the last sequence are never
 // fetched as columns and whatever they hold cannot reach a gradient.
 #include <algorithm>
+#include <atomic>
 
 #include "attn_tmem.cuh"
 #include "pe_host.h"
@@ -47,6 +48,10 @@ constexpr int BW_PRODUCER = BW_COMPUTE_WARPS;
 constexpr int BW_MMA = BW_COMPUTE_WARPS + 1;
 constexpr int BW_STORER = BW_COMPUTE_WARPS + 4;       // first of four (two in between idle: registers move by fours)
 constexpr int BW_THREADS = 32 * (BW_COMPUTE_WARPS + 8);
+// Registers per thread: what the launch gives (65,536 / 640, in eights) and what each role moves to.
+constexpr int BW_REGS = 96, BW_REGS_COMPUTE = 120, BW_REGS_FEED = 48, BW_REGS_STORE = 72;
+static_assert(BW_COMPUTE_WARPS * BW_REGS_COMPUTE + 4 * BW_REGS_FEED + 4 * BW_REGS_STORE ==
+                  (BW_COMPUTE_WARPS + 8) * BW_REGS, "an increase waits until the others have released as many");
 constexpr int BW_TILE = 128;                        // rows of a row tile
 constexpr int BW_COLS = 64;                         // columns of a column tile
 constexpr int BW_A_BYTES = BW_TILE * 64 * 2;        // one operand of a row tile
@@ -861,13 +866,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
   int second = int(blockIdx.x) - a.n_items % int(gridDim.x);
   if (second < 0) second += gridDim.x;
   if (warp < BW_COMPUTE_WARPS) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BW_REGS_COMPUTE));
     bw_both<BW_COMPUTE>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, second, base, bar_base, tmem_base);
   } else if (warp < BW_STORER) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_REGS_FEED));
     bw_both<BW_FEED>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, second, base, bar_base, tmem_base);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_REGS_STORE));
     bw_both<BW_STORE>(tm_qkv, tm_qkv_cols, tm_dout, tm_dout_cols, a, second, base, bar_base, tmem_base);
   }
   tc_fence_before();
@@ -940,6 +945,16 @@ extern "C" int pe_attn_varlen_backward(const void* dout, const void* qkv, const 
   if (rc != PE_OK) return rc;
   rc = set_max_dynamic_smem(reinterpret_cast<const void*>(attn_bwd_kernel), BW_SMEM, true);
   if (rc != PE_OK) return rc;
+  // A build that needed fewer registers at launch would leave the increase above waiting for good.
+  static std::atomic<int> launch_regs{0};
+  if (launch_regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes attr;
+    PE_CUDA(cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(attn_bwd_kernel)));
+    launch_regs.store(attr.numRegs, std::memory_order_relaxed);
+  }
+  PE_REQUIRE(launch_regs.load(std::memory_order_relaxed) == BW_REGS,
+             "pe_attn_varlen_backward: built with %d registers per thread instead of %d",
+             launch_regs.load(std::memory_order_relaxed), BW_REGS);
   BwArgs a;
   a.row_range = reinterpret_cast<const int2*>(ws + w.row_range);
   a.tile_range = reinterpret_cast<const int2*>(ws + w.tile_range);

@@ -317,6 +317,12 @@ def _attention_args(qkv: Tensor, cu_seqlens: Tensor, n_heads: int, half_window: 
     return _aligned(qkv), cu
 
 
+def _window(half_window: int | None, total: int) -> int:
+    """As the library takes it: -1 for none, and not much wider than any sequence can need (full
+    attention's kernel walks the whole band, also where it leaves the sequence)."""
+    return -1 if half_window is None else min(int(half_window), max(total, 4096))
+
+
 def _aligned(t: Tensor) -> Tensor:
     """The kernels move 16 bytes at a time: a view that starts elsewhere is copied."""
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -336,11 +342,13 @@ def attention_varlen_qkv_lse(qkv: Tensor, cu_seqlens: Tensor, max_seqlen: int, n
     lse = torch.empty(n_heads, total, dtype=torch.float32, device=qkv.device)
     if total == 0:
         return out, lse
+    # grids are sized by it; the floor is far above where it chooses a kernel
+    longest = min(int(max_seqlen), max(total, 65536))
     with _Call(qkv) as c:
         ws_bytes = int(c.lib.pe_attn_workspace_bytes(total, n_seqs))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
         _lib.check(c.lib.pe_attn_varlen_lse(qkv.data_ptr(), cu.data_ptr(), n_seqs, total, n_heads,
-                                            -1 if half_window is None else half_window, int(max_seqlen),
+                                            _window(half_window, total), longest,
                                             out.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes,
                                             status_word(qkv.device).data_ptr(), c.stream),
                    "pe_attn_varlen_lse")
@@ -388,7 +396,7 @@ def attention_varlen_qkv_backward(dout: Tensor, qkv: Tensor, out: Tensor, lse: T
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qkv.device)
         _lib.check(c.lib.pe_attn_varlen_backward(
             dout.data_ptr(), qkv.data_ptr(), out.data_ptr(), lse.data_ptr(), cu.data_ptr(), cu.numel() - 1, total,
-            n_heads, -1 if half_window is None else half_window, _lib.ptr(pos), _lib.ptr(table),
+            n_heads, _window(half_window, total), _lib.ptr(pos), _lib.ptr(table),
             0 if table is None else table.shape[0], dqkv.data_ptr(), ws.data_ptr(), ws_bytes,
             status_word(qkv.device).data_ptr(), c.stream), "pe_attn_varlen_backward")
     return dqkv

@@ -282,7 +282,8 @@ size_t pe_attn_backward_workspace_bytes(int64_t T, int nh);
  * table and position_ids (both or neither): the rotation table and positions that the forward's q
  * and k were rotated with; dq and dk are then turned back, i.e. dqkv is the gradient with respect to
  * the qkv before pe_rope_qk_inplace.  A position outside the table counts as 0 (status 302).  The
- * values of rows behind the last sequence are never read into another row's gradient. */
+ * values of rows behind the last sequence are never read into another row's gradient; as in the
+ * forward, those of another sequence, or of keys outside the window, are multiplied by zero. */
 int pe_attn_varlen_backward(const void* dout, const void* qkv, const void* out, const float* lse,
                             const int32_t* cu_seqlens, int n_seqs, int64_t T, int nh, int half_window,
                             const int64_t* position_ids, const void* table, int max_positions, void* dqkv,
