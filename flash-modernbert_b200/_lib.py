@@ -112,6 +112,7 @@ PROTOTYPES = {
                                       c_void_p, c_void_p]),
     "pe_attn_varlen_lse": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p,
                                    c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "pe_rope_qk": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "pe_attn_backward_workspace_bytes": (c_size_t, [c_int64, c_int]),
     "pe_attn_varlen_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
                                         c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,

@@ -105,8 +105,6 @@ __device__ __forceinline__ void dropout_octet(float (&v)[8], const float (&r)[8]
 
 // VECTOR: every pointer is 16-byte aligned, whole octets move in 16-byte pieces (the last, partial one
 // element by element).  threshold_hi: the drop threshold times 2^16; `all`: everything is dropped.
-// VECTOR: every pointer is 16-byte aligned, whole octets move in 16-byte pieces (the last, partial one
-// element by element).  threshold_hi: the drop threshold times 2^16; `all`: everything is dropped.
 // Eight blocks per SM, all 64 warps, hide the generator's latency; two octets per thread and step, or the next
 // octet's loads issued a step ahead, cost the registers that the warps need and were slower
 // (306,851 x 768 bf16: 193 us as it is, 196 - 212 us so).

@@ -402,11 +402,27 @@ def attention_varlen_qkv_backward(dout: Tensor, qkv: Tensor, out: Tensor, lse: T
     return dqkv
 
 
+def rope_qk(qkv: Tensor, position_ids: Tensor, table: Tensor, n_heads: int) -> Tensor:
+    """`rope_qk_inplace` into a new tensor: one pass that reads `qkv` and writes it with q and k rotated."""
+    qkv = _bf16_cuda(qkv, "qkv")
+    if n_heads <= 0 or qkv.dim() != 2 or qkv.shape[1] != 3 * n_heads * 64:
+        raise ValueError(f"qkv must be [T, 3 * {n_heads} * 64], got {tuple(qkv.shape)}")
+    pos, table = _rotation_args(position_ids, table, qkv)
+    if table is None:
+        raise ValueError("rope_qk needs position_ids and table")
+    qkv = _aligned(qkv)
+    out = torch.empty_like(qkv)
+    with _Call(qkv) as c:
+        _lib.check(c.lib.pe_rope_qk(qkv.data_ptr(), pos.data_ptr(), table.data_ptr(), table.shape[0], qkv.shape[0],
+                                    n_heads, out.data_ptr(), status_word(qkv.device).data_ptr(), c.stream), "pe_rope_qk")
+    return out
+
+
 class _AttentionVarlen(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, cu_seqlens, max_seqlen, n_heads, half_window, position_ids, table):
         if table is not None:
-            qkv = rope_qk_inplace(qkv.detach().clone(memory_format=torch.contiguous_format), position_ids, table, n_heads)
+            qkv = rope_qk(qkv.detach(), position_ids, table, n_heads)
         out, lse = attention_varlen_qkv_lse(qkv, cu_seqlens, max_seqlen, n_heads, half_window)
         ctx.save_for_backward(qkv, out, lse, cu_seqlens, position_ids, table)
         ctx.sizes = (max_seqlen, n_heads, half_window)

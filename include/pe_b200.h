@@ -271,6 +271,11 @@ int pe_attn_varlen_lse(const void* qkv, const int32_t* cu_seqlens, int n_seqs, i
                        int half_window, int max_seqlen, void* out, float* lse, void* workspace,
                        size_t workspace_bytes, int32_t* status, void* stream);
 
+/* pe_rope_qk_inplace into another buffer: out, bf16 [T, 3*nh*64], receives q and k turned and v as it is,
+ * the same bits as a copy of qkv rotated in place.  All pointers 16-byte aligned, out not qkv. */
+int pe_rope_qk(const void* qkv, const int64_t* position_ids, const void* table, int max_positions,
+               int64_t T, int nh, void* out, int32_t* status, void* stream);
+
 /* Bytes of scratch pe_attn_varlen_backward needs for T tokens and nh heads. */
 size_t pe_attn_backward_workspace_bytes(int64_t T, int nh);
 
