@@ -16,8 +16,8 @@
 // eight CTAs that each take a part of the vocabulary and join through distributed shared memory.
 //
 // Top k: the pass also leaves, in shared memory, the largest of every sixteen logits (or multiple of
-// sixteen) that a thread has read.  A threshold follows from them at once: the k / 8-th largest (rounded
-// up) of a warp's 32 thread maxima, the least of these over the eight warps - at least k logits
+// sixteen) that a thread has read.  A threshold follows from them at once: the k / W-th largest (rounded
+// up) of a warp's 32 thread maxima, the least of these over the W warps - at least k logits
 // reach it.  Only the sixteens whose largest reaches the threshold are read again, some tens of 3,000 in a
 // row of 50,368, and what reaches the threshold in them is pushed into a small list.  Order is total:
 // a candidate is the 64-bit number (value's bits made monotone, complement of the index), so
@@ -92,11 +92,11 @@ __device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b) {
   return r;
 }
 
-constexpr int LP_TOPS = 16;  // maxima that a thread leaves behind (sixteens are joined beyond 65,536 logits per CTA)
+constexpr int LP_TOPS = 16;  // maxima that a thread leaves behind; beyond, sixteens are joined
 
 template <int NT, bool TOP>
 struct LpShared {
-  static constexpr int CAP = 1536;  // list of candidates; a round adds at most 16 * LP_CROWD = 512
+  static constexpr int CAP = 16 * LP_CROWD + 4 * NT;  // list of candidates; a round adds at most 16 * LP_CROWD
   LpStat stat[NT / 32];
   LpStat part[LP_MAX_CLUSTER];                       // parts of the cluster's CTAs, in rank 0
   float lse[2];
@@ -173,8 +173,10 @@ __device__ __forceinline__ float lp_top(const uint4 (&u)[VECS]) {
   }
 }
 
+// Registers: for 1,280 threads per SM (48 each); fp32 with the top for 1,024 (64), which was faster there
+// (515 x 256,001, top five: 97 us against 100; 16-bit types the other way, 8,192 x 50,368: 243 against 221).
 template <typename E, int NT, bool TOP>
-__global__ void __launch_bounds__(NT, TOP ? 4 : 5)
+__global__ void __launch_bounds__(NT, (TOP && sizeof(E) == 4 ? 4 : 5) * (256 / NT))
 token_logprobs_kernel(const LpArgs a, int cluster) {
   constexpr int N = LogitVec<E>::N;
   constexpr int VECS = 16 / N;  // 16-byte loads per thread and chunk: 16 logits
@@ -222,15 +224,19 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
   const uint32_t lowest = sizeof(E) == 4 ? 0xff800000u : (std::is_same<E, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
   uint4 next[VECS];
   auto load = [&](int v0) {
+    const uint4* at = xv + v0 + tid;
+    if (v0 + CHUNK <= v_end) {  // the same for the whole CTA: only the last chunk asks vector by vector
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int v = v0 + i * NT + tid;
-      next[i] = v < v_end ? ld_stream(xv + v) : make_uint4(lowest, lowest, lowest, lowest);
+      for (int i = 0; i < VECS; ++i) next[i] = ld_stream(at + i * NT);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VECS; ++i)
+        next[i] = v0 + i * NT + tid < v_end ? ld_stream(at + i * NT) : make_uint4(lowest, lowest, lowest, lowest);
     }
   };
   if (chunks > 0) load(v_begin);
   float joined = -INFINITY;
-  int filled = 0;
+  int filled = 0, kept_rows = 0;  // chunks in `joined`, rows of sh.tops written
   for (int c = 0; c < chunks; ++c) {
     const float top = lp_top<E, VECS>(next);
     float f[VECS][N];
@@ -240,7 +246,7 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
     if (TOP) {
       joined = lp_max_nan(joined, top);
       if (++filled == join || c + 1 == chunks) {
-        sh.tops[c / join][tid] = joined;
+        sh.tops[kept_rows++][tid] = joined;
         joined = -INFINITY;
         filled = 0;
       }
@@ -278,8 +284,9 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
   }
 
   if (TOP) {
-    // Threshold: from the warps whose lanes all have logits, so that at least k reach it (none: 0).
-    const int full_warps = min(WARPS, (v_end - v_begin) / 32);
+    // Threshold: from the warps whose lanes all have logits (or the first, if k of its lanes have some), so that
+    // at least k reach it (none: 0).
+    const int full_warps = max(min(WARPS, (v_end - v_begin) / 32), v_end - v_begin >= k ? 1 : 0);
     {
       const int lane = tid & 31;
       uint32_t mine = uint32_t(lp_key(st.m, 0) >> 32), level = 0u;
@@ -297,11 +304,14 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
     // what equals the threshold may be pushed too
     unsigned long long tau = level == 0u ? 0ull : (static_cast<unsigned long long>(level) << 32) - 1ull;
     // The usual way: list the sixteens that reach tau, then read them all at once, one to a thread.
-    for (int r = 0; r < chunks; ++r)
-      if (v_begin + r * CHUNK + tid < v_end && lp_key(sh.tops[r / join][tid], 0u) > tau) {
-        const int at = atomicAdd(&sh.n_again, 1);
-        if (at < 2 * NT) sh.again[at] = uint32_t(r) * NT + tid;
-      }
+    const float reach = level == 0u ? -INFINITY : lp_key_value(static_cast<unsigned long long>(level) << 32);
+    for (int q = 0; q < kept_rows; ++q)
+      if (!(sh.tops[q][tid] < reach))  // (or a NaN)
+        for (int r = q * join; r < min(chunks, (q + 1) * join); ++r)
+          if (v_begin + r * CHUNK + tid < v_end) {
+            const int at = atomicAdd(&sh.n_again, 1);
+            if (at < 2 * NT) sh.again[at] = uint32_t(r) * NT + tid;
+          }
     auto push = [&](unsigned long long key) {
       if (key > tau) {
         const int at = atomicAdd(&sh.count, 1);
@@ -586,9 +596,8 @@ token_logprobs_backward_kernel(const LpBackArgs a, int64_t rows) {
   }
 }
 
-template <typename E>
+template <typename E, int NT>
 static int launch_logprobs(const LpArgs& a, int64_t rows, cudaStream_t st) {
-  constexpr int NT = 256;
   auto kern = a.top_k > 0 ? token_logprobs_kernel<E, NT, true> : token_logprobs_kernel<E, NT, false>;
   // A row is split over a cluster while the rows alone leave SMs idle and a CTA keeps at least one
   // full chunk (4,096 logits) of work.
@@ -654,10 +663,15 @@ extern "C" int pe_token_logprobs(const void* logits, int dtype, int64_t rows, in
   const LpArgs a{logits, ld, targets, ignore_index, (int)vocab, top_k, logprobs, entropy, lse, lse_rest, top_ids,
                  top_logprobs, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // 128 threads to a row where the rows fill the GPU several times over: half as much joining and selecting
+  // per row (8,192 x 50,368 bf16: 157 us against 165, with the top five 202 against 221; 16,384 x 8,000
+  // 73 against 91, 134 against 181).  With fewer rows, or sixteens joined too often for the top, 256
+  // (515 x 256,001 fp32: 88 us against 109, with the top five 94 against 254).
+  const bool many = rows >= 6 * int64_t(sm_count()) && (top_k == 0 || vocab <= 65536);
   switch (dtype) {
-    case PE_BF16: return launch_logprobs<__nv_bfloat16>(a, rows, st);
-    case PE_FP16: return launch_logprobs<__half>(a, rows, st);
-    default: return launch_logprobs<float>(a, rows, st);
+    case PE_BF16: return many ? launch_logprobs<__nv_bfloat16, 128>(a, rows, st) : launch_logprobs<__nv_bfloat16, 256>(a, rows, st);
+    case PE_FP16: return many ? launch_logprobs<__half, 128>(a, rows, st) : launch_logprobs<__half, 256>(a, rows, st);
+    default: return many ? launch_logprobs<float, 128>(a, rows, st) : launch_logprobs<float, 256>(a, rows, st);
   }
 }
 
