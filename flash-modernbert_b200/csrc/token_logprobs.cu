@@ -340,9 +340,11 @@ token_logprobs_kernel(const LpArgs a, int cluster) {
     }
     __syncthreads();
     const bool crowded = n_again > 2 * NT || sh.count > LpShared<NT, TOP>::CAP;  // the same for every thread
-    __syncthreads();
-    if (crowded && tid == 0) sh.count = 0;
-    __syncthreads();
+    if (crowded) {
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+    }
     // Otherwise, whatever the data, in rounds of bounded size.
     // Round r < chunks: sixteen logits of every thread whose maximum is not below tau; the last round:
     // the odd ones.
