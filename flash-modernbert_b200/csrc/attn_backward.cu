@@ -16,13 +16,13 @@
 // from tensor memory (the A operand of tcgen05.mma), and no score ever passes through shared
 // memory.  The price against one pass that would add dQ tiles into global memory is a second S, dP
 // and exponential (seven products instead of five); what it buys is a fixed summation order and
-// no fp32 dQ buffer: that one pass moves 32 KB of fp32 additions through L2 per tile of 1,280
-// tensor clocks, 25 B per clock and SM, more than L2 takes.
+// no fp32 dQ buffer: that one pass moves 32 KB of fp32 additions through L2 per 128 x 128 scores, 25 B
+// per clock and SM at the tensor cores' pace, more than L2 takes.
 //
 // Rows are tiled over the packed tokens, not per sequence: a tile of 128 consecutive tokens may
 // hold many sequences.  Row i attends the columns [lo_i, hi_i) - its sequence, cut to the window -
 // and the relation is symmetric, so the same two numbers serve both passes.  A batch of 30-token
-// queries then costs one 128-column tile per four queries instead of one each.  A tile walks the
+// queries then costs one row tile per four queries instead of one each.  A tile walks the
 // columns [min lo, max hi) of its rows; its last column tile ends exactly at max hi (it overlaps the
 // one before, whose columns are masked out there), so rows behind the last sequence are never
 // fetched as columns and whatever they hold cannot reach a gradient.
