@@ -224,20 +224,6 @@ struct BwItem {
   __device__ __forceinline__ int col0(int j) const { return j + 1 == n ? hi - BW_COLS : lo + j * BW_COLS; }
 };
 
-// A waiting instruction takes about a hundred clocks to answer even when its phase is complete.  This one does
-// not wait: it is issued ahead of other work, and only where its answer, read after that work, is "not
-// yet" does a wait follow.
-__device__ __forceinline__ bool bw_test(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, P;\n\t}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
 // Bounded: the instruction itself waits up to about half a microsecond, so this gives up after seconds at most.
 __device__ __forceinline__ bool bw_wait(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -671,7 +657,6 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
     auto wait = [&](int b, uint32_t parity) {
       if (ok) ok = bw_wait(bar(b), parity);
     };
-    auto test = [&](int b, uint32_t parity) { return bw_test(bar(b), parity); };
     auto arrive = [&](int b) {
       tc_fence_before();
       __syncwarp();
@@ -699,14 +684,13 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
           const uint32_t s_addr = lane_addr + c * 64;
           const uint32_t dp_addr = s_addr ^ 64u;
           const uint32_t stats = sStats + c * BW_STATS_BYTES;
-          const bool s_full = test(WB_S_FULL + c, lap), b_full = !KEYS || test(WB_IN + c, lap);
+          if (KEYS) wait(WB_IN + c, lap);  // long complete: makes lse and delta visible
           // valid columns of this row within the tile: [c_lo, c_hi)
           const int x0 = it.col0(j);
           const int c_lo = max(range.x, it.lo + j * BW_COLS) - x0, c_hi = range.y - x0;
           const bool full = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= BW_COLS);
           const bool none = __all_sync(0xffffffffu, c_lo >= c_hi || c_hi <= 0 || c_lo >= BW_COLS);
-          if (!s_full) wait(WB_S_FULL + c, lap);
-          if (!b_full) wait(WB_IN + c, lap);  // complete by now: makes lse and delta visible
+          wait(WB_S_FULL + c, lap);
           tc_fence_after();
           if (none) {  // no row of this warp attends any of the columns
             uint32_t zero[16];
@@ -720,7 +704,6 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
             g_tmem_ld32(s_addr, p);
             tmem_ld_wait();
             g_tmem_ld32(s_addr + 32, p + 32);  // in flight during the first half's exponentials
-            const bool dp_full = test(WB_DP_FULL + c, lap);
             auto exponentials = [&](int e0) {
 #pragma unroll
               for (int e = e0; e < e0 + 32; e += 4) {
@@ -759,7 +742,7 @@ __device__ __forceinline__ bool bw_pass(const CUtensorMap& tm_qkv, const CUtenso
                 g_tmem_st16(s_addr + h * 16, pk);
               }
             }
-            if (!dp_full) wait(WB_DP_FULL + c, lap);
+            wait(WB_DP_FULL + c, lap);
             tc_fence_after();
             uint32_t dp[2][16];
             g_tmem_ld16(dp_addr, dp[0]);
